@@ -83,6 +83,7 @@ struct CnnLane {
     hipStream_t stream = nullptr;
     std::mutex mu;                                       // enqueue order == execution order
     DevBuf buf[8], valid, enclen, enchist, permsrc, permrow, live;
+    DevBuf canary;                                       // the canary's probabilities (cnn_execute): written and read on this stream only, gone with the lane
     size_t bytes = 0;
     int users = 0;                                       // guarded by g_lane_mu: passes that hold `mu` or are about to take it (lane_get .. lane_put)
 };
@@ -105,7 +106,7 @@ static int lanes_free_device(int dev) {
         (void)hipSetDevice(dev);
         if (L->stream) { (void)hipStreamSynchronize(L->stream); (void)hipStreamDestroy(L->stream); }
         for (DevBuf &b : L->buf) if (b.p) (void)hipFree(b.p);
-        for (DevBuf *b : { &L->valid, &L->enclen, &L->enchist, &L->permsrc, &L->permrow, &L->live }) if (b->p) (void)hipFree(b->p);
+        for (DevBuf *b : { &L->valid, &L->enclen, &L->enchist, &L->permsrc, &L->permrow, &L->live, &L->canary }) if (b->p) (void)hipFree(b->p);
         g_lane[dev][l] = nullptr;                        // nobody can find the lane any more (lookups go through g_lane under g_lane_mu) ...
         L->mu.unlock();
         delete L;                                        // ... so nobody can be waiting on its mutex
@@ -173,7 +174,7 @@ struct dn_ctx {
     std::vector<int64_t> cnn_wb_off, cnn_wh_off; uint16_t *d_cnn_wb = nullptr, *d_cnn_wh = nullptr; size_t cnn_nwb = 0, cnn_nwh = 0; int cnn_math = DN_CNN_MATH_F16X3;
     std::vector<float> cnn_post, cnn_one; unsigned *d_cnn_flag = nullptr; uint64_t cnn_escalations = 0; bool cnn_f16_off = false;
     unsigned cnn_underflow_streak = 0; bool cnn_bf16_once = false;        // see cnn_note_escalation
-    DevBuf cnn_canary; uint64_t cnn_canaries = 0;                         // the canary's probabilities (cnn_execute); how many canaries ran
+    uint64_t cnn_canaries = 0;                                            // how many canaries ran
     std::vector<dn_cnn_op> cnn_ops; float *d_cnn_w = nullptr; size_t cnn_nw = 0; int cnn_nbuf = 0; DevBuf cnn_rowoff, cnn_npos, cnn_iooff, cnn_in[3], cnn_out;
     hipEvent_t ev_ready = nullptr, ev_done = nullptr;    // hand-over to / from the device's CNN lane
     unsigned lane_id = 0;
@@ -489,7 +490,7 @@ void dn_ctx_destroy(dn_ctx *c) {
     for (auto *p : c->d_fit) if (p) hipFree(p);
     for (DevBuf *b : { &c->hmm_poi, &c->hmm_npoi, &c->hmm_nev, &c->hmm_ok, &c->hmm_la, &c->hmm_lt, &c->hmm_reads, &c->al_coord, &c->al_rpos,
                        &c->al_val, &c->al_kind, &c->al_off, &c->al_n }) if (b->p) hipFree(b->p);
-    for (DevBuf *b : { &c->cnn_rowoff, &c->cnn_npos, &c->cnn_iooff, &c->cnn_in[0], &c->cnn_in[1], &c->cnn_in[2], &c->cnn_out, &c->cnn_canary }) if (b->p) hipFree(b->p);
+    for (DevBuf *b : { &c->cnn_rowoff, &c->cnn_npos, &c->cnn_iooff, &c->cnn_in[0], &c->cnn_in[1], &c->cnn_in[2], &c->cnn_out }) if (b->p) hipFree(b->p);
     if (c->ev_ready) hipEventDestroy(c->ev_ready);
     if (c->ev_done) hipEventDestroy(c->ev_done);
     if (c->own_stream) hipStreamDestroy(c->stream);
@@ -1524,11 +1525,11 @@ static int cnn_execute(dn_ctx *c, uint32_t n, const unsigned *ub, const unsigned
                 while (k1 < ps.r1 && k1 - ps.r0 < 8 && cpos < 4096) { crows += ub[k1] + 8; cpos += ub[k1]; cmax = std::max(cmax, ub[k1]); k1++; }
                 const uint64_t span = io_off[k1 - 1] + ub[k1 - 1] - io_off[ps.r0];                 // positions from the first canary sequence's first to the last one's bound
                 // (sized once for any read up to 512 k positions: regrowing frees, and hipFree waits for the whole device -- every batch in flight drained)
-                if ((rc = dgrow(c, c->cnn_canary, (size_t)std::max<uint64_t>(span, 512u << 10) * 3 * sizeof(float)))) return rc;
+                if ((rc = lane_grow(c, L, L->canary, (size_t)std::max<uint64_t>(span, 512u << 10) * 3 * sizeof(float)))) return rc;
                 CnnRun cr = run;
                 cr.rows.r1 = k1; cr.rows.rows = (unsigned)((crows + 255) / 256 * 256); cr.max_pos = cmax; cr.n_pass_pos = (unsigned)cpos;
                 cr.wts_split = c->d_cnn_wb; cr.wb_off = c->cnn_wb_off.data(); cr.pieces = 3; cr.post = c->cnn_one.data();
-                cr.probs = (float *)c->cnn_canary.p - 3 * io_off[ps.r0];                            // k3_dense_softmax writes at probs + 3 (io_off[r] + p)
+                cr.probs = (float *)L->canary.p - 3 * io_off[ps.r0];                            // k3_dense_softmax writes at probs + 3 (io_off[r] + p)
                 cr.mark = nullptr;
                 HIPCHK(c, hipMemsetAsync(L->valid.p, 0, (size_t)ps.rows, st));
                 if (k3_run(cr, st)) return fail(c, DN_ERR_ARG, "unsupported op in the CNN description");
