@@ -1059,11 +1059,30 @@ int dn_host_alloc(size_t bytes, void **p) {
     return hipHostMalloc(p, std::max<size_t>(bytes, 1), hipHostMallocDefault) == hipSuccess ? DN_OK : DN_ERR_HIP;
 }
 void dn_host_free(void *p) { if (p) (void)hipHostFree(p); }
+// Some systems refuse to page-lock memory that exists already.  The arrays then stay pageable: dn_batch_upload asks every pointer what it is and
+// waits for its copies.  The refused pointers are kept so that dn_host_unregister answers for them as for the others.
+static std::mutex g_pageable_mu;
+static std::vector<void *> g_pageable;
 int dn_host_register(void *p, size_t bytes) {
     if (!p || !bytes) return DN_ERR_ARG;
-    return hipHostRegister(p, bytes, hipHostRegisterDefault) == hipSuccess ? DN_OK : DN_ERR_HIP;
+    if (hipHostRegister(p, bytes, hipHostRegisterDefault) == hipSuccess) return DN_OK;
+    (void)hipGetLastError();                               // the refusal must not surface after the next launch
+    std::lock_guard<std::mutex> lk(g_pageable_mu);
+    if (g_pageable.empty()) fprintf(stderr, "dnascent_hip: the system does not page-lock existing memory; uploads from it wait for their copies\n");
+    g_pageable.push_back(p);
+    return DN_OK;
 }
-int dn_host_unregister(void *p) { return (p && hipHostUnregister(p) == hipSuccess) ? DN_OK : DN_ERR_HIP; }
+int dn_host_unregister(void *p) {
+    if (!p) return DN_ERR_HIP;
+    {
+        std::lock_guard<std::mutex> lk(g_pageable_mu);
+        const auto it = std::find(g_pageable.begin(), g_pageable.end(), p);
+        if (it != g_pageable.end()) { g_pageable.erase(it); return DN_OK; }
+    }
+    if (hipHostUnregister(p) == hipSuccess) return DN_OK;
+    (void)hipGetLastError();
+    return DN_ERR_HIP;
+}
 
 #define CHECK_READ(stage_, name_)                                     \
     int rc = need(c, stage_, name_); if (rc) return rc;              \

@@ -87,7 +87,9 @@ typedef struct {
  * With page-locked input arrays (dn_host_alloc / dn_host_register) the copies themselves are asynchronous too and the arrays
  * must stay untouched until the next dn_sync / dn_collect of this context; with pageable arrays the call returns after the copies. */
 int dn_batch_upload(dn_ctx *ctx, const dn_batch_desc *batch);
-/* page-locked host memory for the input arrays: hipHostMalloc / hipHostRegister behind a C signature */
+/* page-locked host memory for the input arrays: hipHostMalloc / hipHostRegister behind a C signature.  Where the system refuses to
+ * page-lock memory that exists already, dn_host_register still returns DN_OK: the memory stays pageable and uploads from it wait for
+ * their copies (dn_batch_upload asks every pointer); memory that must be page-locked comes from dn_host_alloc. */
 int dn_host_alloc(size_t bytes, void **p);
 void dn_host_free(void *p);
 int dn_host_register(void *p, size_t bytes);
