@@ -7,6 +7,7 @@
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -15,7 +16,8 @@ LIB = os.path.join(HERE, "lib")
 HIP_SO = os.path.join(LIB, "libdnascent_hip.so")
 HOST_SO = os.path.join(LIB, "libdnascent_host.so")
 
-HIP_SOURCES = ["dn_capi.hip", "k1_segment.hip", "k2_banded.hip", "k_scaling.hip", "k2b_viterbi.hip", "k3_cnn.hip", "k_hmm.hip", "k_collect.hip"]
+HIP_SOURCES = ["dn_capi.hip", "k1_segment.hip", "k2_banded.hip", "k_scaling.hip", "k2b_viterbi.hip", "k3_cnn.hip", "k_hmm.hip", "k_collect.hip", "k8_dense.hip"]
+PACKED_FP32 = {"k3_cnn.hip"}                              # writes packed fp32 instructions by hand; everywhere else the compiler makes none
 HOST_SOURCES = ["host/dn_synth.c", "host/dn_host.cpp", "host/dn_bam.cpp", "host/dn_vbz.cpp"]       # dn_bam.cpp: BGZF / BAM over zlib (libz is in the image; htslib is not); dn_vbz.cpp: POD5's signal codec (zstd through dlopen)
 
 
@@ -47,11 +49,19 @@ def build_hip(force=False):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     # -ffp-contract=off: the reference arithmetic has no FMA contraction (Makefile:6 plain -O2 on x86-64);
     # every fused multiply-add in the kernels is written explicitly.
-    cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off",
-           "-fno-fast-math", "-Wall", "-Wno-unused-function", "-Wno-unused-value", "-Wno-unused-result",
-           "-fhip-fp32-correctly-rounded-divide-sqrt",
-           "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-o", HIP_SO] + os.environ.get("DN_HIPCC_FLAGS", "").split() + srcs   # DN_HIPCC_FLAGS: experiment builds (-DDN_WS_TRACE=<workgroup>)
-    _run(cmd)
+    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
+             "-fno-fast-math", "-Wall", "-Wno-unused-function", "-Wno-unused-value", "-Wno-unused-result",
+             "-fhip-fp32-correctly-rounded-divide-sqrt",
+             "-I", os.path.join(ROOT, "include"), "-I", CSRC] + os.environ.get("DN_HIPCC_FLAGS", "").split()   # DN_HIPCC_FLAGS: experiment builds (-DDN_WS_TRACE=<workgroup>)
+    objs, jobs = [], []
+    for s in srcs:
+        o = os.path.join(LIB, os.path.basename(s) + ".o")
+        unpacked = [] if os.path.basename(s) in PACKED_FP32 else ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+        jobs.append([hipcc] + flags + unpacked + ["-c", s, "-o", o])
+        objs.append(o)
+    with ThreadPoolExecutor(min(len(jobs), int(os.environ.get("MAX_JOBS", "6")))) as pool:
+        list(pool.map(_run, jobs))
+    _run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", HIP_SO] + objs)
     return HIP_SO
 
 

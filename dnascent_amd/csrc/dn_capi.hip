@@ -3,6 +3,7 @@
 // stream and exposes the intermediate taps the parity tests read.  No CPU fallback anywhere.
 #include "dnascent_hip.h"
 #include "dn_dev.h"
+#include "k8_dense.h"
 
 #include <math.h>
 #include <stdarg.h>
@@ -1766,6 +1767,134 @@ int dn_get_hmm_calls(dn_ctx *c, uint32_t read, uint64_t cap, uint32_t *pos_on_re
         if (llr) llr[o] = a - t;
         o++;
     }
+    return DN_OK;
+}
+
+// ---- 8-bit dense layers (k8_dense.hip) on the caller's device memory and stream ----
+// the caller's current device comes back however the call ends
+struct DeviceScope {
+    int before = -1, want; hipError_t e = hipSuccess;
+    explicit DeviceScope(int device) : want(device) {
+        e = hipGetDevice(&before);
+        if (e == hipSuccess && before != want) e = hipSetDevice(want);
+    }
+    ~DeviceScope() { if (before >= 0 && before != want) (void)hipSetDevice(before); }
+    DeviceScope(const DeviceScope &) = delete; DeviceScope &operator=(const DeviceScope &) = delete;
+};
+static bool t_number(int t) { return t == DN_T_F32 || t == DN_T_F16 || t == DN_T_BF16; }
+static unsigned t_bytes(int t) { return t == DN_T_F32 ? 4u : t == DN_T_I8 ? 1u : 2u; }
+// a matrix argument: there (unless it has no rows), on its type's boundary, rows that hold `cols` elements (ld 0: one row for all, inputs only)
+static bool t_matrix(const void *p, int64_t rows, int64_t cols, int64_t ld, unsigned bytes, bool output) {
+    if (rows == 0) return true;
+    if (!p || (uintptr_t)p % bytes) return false;
+    if (ld < 0 || ld >= (1ll << 31)) return false;
+    return ld >= cols || (rows == 1 && !output) || (!output && ld == 0);
+}
+static int i8_sizes(dn_ctx *c, const char *what, int64_t m, int64_t n, int64_t k) {
+    if (m < 0 || m >= DN_I8_MAX_M) return fail(c, DN_ERR_ARG, "%s: %lld rows", what, (long long)m);
+    if (n < 1 || n > DN_I8_MAX_K || k < 1 || k > DN_I8_MAX_K) return fail(c, DN_ERR_ARG, "%s: %lld x %lld channels (1 .. %d)", what, (long long)k, (long long)n, DN_I8_MAX_K);
+    return DN_OK;
+}
+#define I8_DEVICE(c)                                                                                                       \
+    DeviceScope scope((c)->device);                                                                                        \
+    if (scope.e != hipSuccess) return fail((c), DN_ERR_HIP, "hipSetDevice(%d): %s", (c)->device, hipGetErrorString(scope.e))
+#define I8_MATRIX(what, name, p, rows, cols, ld, bytes, output)                                                            \
+    if (!t_matrix((p), (rows), (cols), (ld), (bytes), (output))) return fail(c, DN_ERR_ARG, "%s: %s is missing, misaligned or has too short a pitch", what, name)
+
+int dn_i8_rows(dn_ctx *c, int64_t m, int64_t k, const void *x, int64_t ldx, int x_type, int8_t *q, int64_t ldq, float *s, void *hip_stream) {
+    if (!c) return DN_ERR_ARG;
+    int rc = i8_sizes(c, "dn_i8_rows", m, 1, k); if (rc) return rc;
+    if (!t_number(x_type)) return fail(c, DN_ERR_ARG, "dn_i8_rows: type %d", x_type);
+    I8_MATRIX("dn_i8_rows", "x", x, m, k, ldx, t_bytes(x_type), false);
+    I8_MATRIX("dn_i8_rows", "q", q, m, k, ldq, 1, true);
+    I8_MATRIX("dn_i8_rows", "s", s, m, 1, 1, 4, true);
+    I8_DEVICE(c);
+    HIPCHK(c, k8_rows(m, k, x, ldx, x_type, q, ldq, s, (hipStream_t)hip_stream));
+    return DN_OK;
+}
+
+int dn_i8_restore(dn_ctx *c, int64_t m, int64_t k, const int8_t *q, int64_t ldq, const float *s, void *x, int64_t ldx, int x_type, void *hip_stream) {
+    if (!c) return DN_ERR_ARG;
+    int rc = i8_sizes(c, "dn_i8_restore", m, 1, k); if (rc) return rc;
+    if (!t_number(x_type)) return fail(c, DN_ERR_ARG, "dn_i8_restore: type %d", x_type);
+    I8_MATRIX("dn_i8_restore", "q", q, m, k, ldq, 1, false);
+    I8_MATRIX("dn_i8_restore", "s", s, m, 1, 1, 4, false);
+    I8_MATRIX("dn_i8_restore", "x", x, m, k, ldx, t_bytes(x_type), true);
+    I8_DEVICE(c);
+    HIPCHK(c, k8_restore(m, k, q, ldq, s, x, ldx, x_type, (hipStream_t)hip_stream));
+    return DN_OK;
+}
+
+static int i8_linear_check(dn_ctx *c, const dn_i8_linear_desc *d) {
+    const char *what = "dn_i8_linear";
+    int rc = i8_sizes(c, what, d->m, d->n, d->k); if (rc) return rc;
+    const bool given = d->x_type == DN_T_I8;
+    if (!given && !t_number(d->x_type)) return fail(c, DN_ERR_ARG, "%s: x type %d", what, d->x_type);
+    if (!t_number(d->y_type)) return fail(c, DN_ERR_ARG, "%s: y type %d", what, d->y_type);
+    if (d->relu < 0 || d->relu > 1 || d->reserved) return fail(c, DN_ERR_ARG, "%s: relu is 0 or 1, reserved is 0", what);
+    if (d->m && given != (d->sx != nullptr)) return fail(c, DN_ERR_ARG, "%s: sx goes with 8-bit rows and with nothing else", what);
+    if (d->mask && !d->relu) return fail(c, DN_ERR_ARG, "%s: a mask without a ReLU", what);
+    if ((d->q != nullptr) != (d->s != nullptr) || (d->q && given)) return fail(c, DN_ERR_ARG, "%s: q and s go together, and with rows that are not in 8 bits yet", what);
+    const unsigned ey = t_bytes(d->y_type);
+    I8_MATRIX(what, "x", d->x, d->m, d->k, d->ldx, t_bytes(d->x_type), false);
+    if (given) I8_MATRIX(what, "sx", d->sx, d->m, 1, 1, 4, false);
+    I8_MATRIX(what, "w", d->w, d->n, d->k, d->ldw, 1, false);
+    I8_MATRIX(what, "sw", d->sw, d->n, 1, 1, 4, false);
+    if (d->bias) I8_MATRIX(what, "bias", d->bias, d->n, 1, 1, 4, false);
+    if (d->residual) I8_MATRIX(what, "residual", d->residual, d->m, d->n, d->ldr, ey, false);
+    I8_MATRIX(what, "y", d->y, d->m, d->n, d->ldy, ey, true);
+    if (d->mask) I8_MATRIX(what, "mask", d->mask, d->m, (d->n + 7) / 8, d->ldmask, 1, true);
+    if (d->q) { I8_MATRIX(what, "q", d->q, d->m, d->k, d->ldq, 1, true); I8_MATRIX(what, "s", d->s, d->m, 1, 1, 4, true); }
+    return DN_OK;
+}
+static int i8_workspace_check(dn_ctx *c, const char *what, const void *ws, uint64_t have, uint64_t need) {
+    if (have < need || (need && (!ws || (uintptr_t)ws % 256))) return fail(c, DN_ERR_ARG, "%s: the workspace needs %llu bytes on a 256-byte boundary (%llu given)", what,
+                                                                          (unsigned long long)need, (unsigned long long)have);
+    return DN_OK;
+}
+int dn_i8_linear_workspace(dn_ctx *c, const dn_i8_linear_desc *d, uint64_t *bytes) {
+    if (!d || !bytes) return DN_ERR_ARG;
+    int rc = i8_linear_check(c, d); if (rc) return rc;
+    *bytes = k8_linear_workspace(*d);
+    return DN_OK;
+}
+int dn_i8_linear(dn_ctx *c, const dn_i8_linear_desc *d, void *workspace, uint64_t workspace_bytes, void *hip_stream) {
+    if (!c || !d) return DN_ERR_ARG;
+    int rc = i8_linear_check(c, d); if (rc) return rc;
+    if ((rc = i8_workspace_check(c, "dn_i8_linear", workspace, workspace_bytes, k8_linear_workspace(*d)))) return rc;
+    I8_DEVICE(c);
+    HIPCHK(c, k8_linear(*d, workspace, (hipStream_t)hip_stream));
+    return DN_OK;
+}
+
+static int i8_grad_check(dn_ctx *c, const dn_i8_grad_desc *d) {
+    const char *what = "dn_i8_linear_grad";
+    int rc = i8_sizes(c, what, d->m, d->n, d->k); if (rc) return rc;
+    if (!t_number(d->dy_type) || !t_number(d->dw_type)) return fail(c, DN_ERR_ARG, "%s: types %d, %d", what, d->dy_type, d->dw_type);
+    if (!d->dx && !d->dw && !d->db && d->m) return fail(c, DN_ERR_ARG, "%s: nothing is asked for", what);
+    I8_MATRIX(what, "dy", d->dy, d->m, d->n, d->ldy, t_bytes(d->dy_type), false);
+    if (d->mask) I8_MATRIX(what, "mask", d->mask, d->m, (d->n + 7) / 8, d->ldmask, 1, false);
+    if (d->dw) { I8_MATRIX(what, "q", d->q, d->m, d->k, d->ldq, 1, false); I8_MATRIX(what, "s", d->s, d->m, 1, 1, 4, false); }
+    if (d->dx) {
+        I8_MATRIX(what, "w", d->w, d->n, d->k, d->ldw, 1, false); I8_MATRIX(what, "sw", d->sw, d->n, 1, 1, 4, false);
+        I8_MATRIX(what, "dx", d->dx, d->m, d->k, d->ldx, t_bytes(d->dy_type), true);
+    }
+    if (d->dw) I8_MATRIX(what, "dw", d->dw, d->n, d->k, d->lddw, t_bytes(d->dw_type), true);
+    if (d->db) I8_MATRIX(what, "db", d->db, d->n, 1, 1, t_bytes(d->dw_type), true);
+    return DN_OK;
+}
+int dn_i8_linear_grad_workspace(dn_ctx *c, const dn_i8_grad_desc *d, uint64_t *bytes) {
+    if (!d || !bytes) return DN_ERR_ARG;
+    int rc = i8_grad_check(c, d); if (rc) return rc;
+    *bytes = k8_grad_workspace(*d);
+    return DN_OK;
+}
+int dn_i8_linear_grad(dn_ctx *c, const dn_i8_grad_desc *d, void *workspace, uint64_t workspace_bytes, void *hip_stream) {
+    if (!c || !d) return DN_ERR_ARG;
+    int rc = i8_grad_check(c, d); if (rc) return rc;
+    if ((rc = i8_workspace_check(c, "dn_i8_linear_grad", workspace, workspace_bytes, k8_grad_workspace(*d)))) return rc;
+    I8_DEVICE(c);
+    HIPCHK(c, k8_grad(*d, workspace, (hipStream_t)hip_stream));
     return DN_OK;
 }
 

@@ -24,7 +24,8 @@ SYMBOLS = ["dn_abi_version", "dn_device_count", "dn_ctx_create", "dn_ctx_destroy
            "dn_run_theilsen", "dn_run_normalise", "dn_run_eventalign", "dn_set_align_table", "dn_get_align_rows", "dn_get_align_table", "dn_load_cnn", "dn_cnn_set_math", "dn_cnn_range_escalations", "dn_cnn_canaries", "dn_run_cnn", "dn_get_probabilities", "dn_cnn_infer", "dn_load_fit_models", "dn_run_hmm", "dn_get_hmm_calls", "dn_get_summaries", "dn_get_prefix_sums",
            "dn_get_tstats", "dn_get_scrappie_events", "dn_get_events", "dn_get_kmer_ranks", "dn_get_alignment",
            "dn_get_cleaned", "dn_get_trace", "dn_get_positions", "dn_get_windows", "dn_profile_enable", "dn_profile_get",
-           "dn_profile_reset", "dn_profile_get_layer", "dn_kernel_name", "dn_device_bytes", "dn_shutdown"]
+           "dn_profile_reset", "dn_profile_get_layer", "dn_kernel_name", "dn_device_bytes", "dn_shutdown",
+           "dn_i8_rows", "dn_i8_restore", "dn_i8_linear_workspace", "dn_i8_linear", "dn_i8_linear_grad_workspace", "dn_i8_linear_grad"]
 
 
 class BatchDesc(C.Structure):
@@ -72,6 +73,21 @@ def cnn_ops_from_description(desc):
         elif o["op"] == "dense_softmax":
             c.src, c.cin, c.cout, c.w, c.shift = o["src"], o["cin"], o["cout"], o["w"], o["b"]
     return ops
+
+
+class I8Linear(C.Structure):
+    """dn_i8_linear_desc"""
+    _fields_ = [("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64), ("sx", C.c_void_p), ("w", C.c_void_p),
+                ("ldw", C.c_int64), ("sw", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("ldr", C.c_int64), ("y", C.c_void_p),
+                ("ldy", C.c_int64), ("mask", C.c_void_p), ("ldmask", C.c_int64), ("q", C.c_void_p), ("ldq", C.c_int64), ("s", C.c_void_p),
+                ("x_type", C.c_int32), ("y_type", C.c_int32), ("relu", C.c_int32), ("reserved", C.c_int32)]
+
+
+class I8Grad(C.Structure):
+    """dn_i8_grad_desc"""
+    _fields_ = [("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("dy", C.c_void_p), ("ldy", C.c_int64), ("mask", C.c_void_p), ("ldmask", C.c_int64),
+                ("q", C.c_void_p), ("ldq", C.c_int64), ("s", C.c_void_p), ("w", C.c_void_p), ("ldw", C.c_int64), ("sw", C.c_void_p), ("dx", C.c_void_p),
+                ("ldx", C.c_int64), ("dw", C.c_void_p), ("lddw", C.c_int64), ("db", C.c_void_p), ("dy_type", C.c_int32), ("dw_type", C.c_int32)]
 
 
 SUMMARY_DTYPE = np.dtype([
@@ -148,6 +164,11 @@ def lib():
         L.dn_device_bytes.restype = C.c_size_t
         L.dn_device_bytes.argtypes = [C.c_void_p]
         L.dn_shutdown.restype = C.c_int
+        L.dn_i8_rows.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]
+        L.dn_i8_restore.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_void_p]
+        for n in ("dn_i8_linear", "dn_i8_linear_grad"):
+            getattr(L, n).argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]
+            getattr(L, n + "_workspace").argtypes = [C.c_void_p, C.c_void_p, C.POINTER(C.c_uint64)]
         _lib = L
     return _lib
 
@@ -166,6 +187,7 @@ class Context:
             raise DnError("dn_ctx_create(device=%d) failed with %d: no usable gfx950 device (no CPU fallback)" % (device, rc))
         self.n_reads = 0
         self._keep = None
+        self.device = int(device)
 
     def _chk(self, rc, what):
         if rc != DN_OK:
@@ -367,6 +389,32 @@ class Context:
         a = np.zeros(n, np.uint32); b = np.zeros(n, np.uint32); t = np.zeros(n, np.uint32); s = np.zeros(n)
         self._chk(lib().dn_get_windows(self.h, r, n, a.ctypes.data, b.ctypes.data, t.ctypes.data, s.ctypes.data), "dn_get_windows")
         return a, b, t, s
+
+    # ---- 8-bit dense layers (dn_i8_*): torch tensors of the context's device, on torch's current stream of that device ---------------
+    def i8_rows(self, x):
+        """dn_i8_rows: x [..., K] (fp32, fp16 or bf16) as rows of 8-bit integers and one fp32 scale each -> (q [..., K] int8, s [...]).  A row of q
+        starts at a multiple of 16 bytes (its pitch is K rounded up), which is how i8_linear and i8_linear_grad read rows fastest; a weight [N, K]
+        becomes (wq, ws) the same way, once."""
+        from . import dense8
+        return dense8.rows(self, x)
+
+    def i8_restore(self, q, s, dtype):
+        """dn_i8_restore: the numbers that i8_rows' result stands for, q * s, rounded once to dtype."""
+        from . import dense8
+        return dense8.restore(self, q, s, dtype)
+
+    def i8_linear(self, x, wq, ws, sx=None, bias=None, residual=None, relu=False, out_dtype=None, save=False):
+        """dn_i8_linear: y [..., N] = act(x W^T + bias + residual) with x [..., K] in 8 bits: numbers (then their rows are made on the way), or int8 rows
+        with their scales sx.  wq [N, K] int8, ws [N] fp32, bias [N] fp32, residual [..., N] of y's type.  out_dtype: x's type, or bf16 for int8 rows.
+        save=True: (y, dense8.Saved) -- what i8_linear_grad needs: the rows, their scales and, with relu, one bit per output."""
+        from . import dense8
+        return dense8.linear(self, x, wq, ws, sx, bias, residual, relu, out_dtype, save)
+
+    def i8_linear_grad(self, dy, q, s, wq, ws, mask=None, need_dx=True, need_dw=True, need_db=True, w_dtype=None):
+        """dn_i8_linear_grad: (dx [..., K] of dy's type, dw [N, K], db [N], both of w_dtype: dy's type if not given) for dy [..., N] from the 8-bit rows
+        of the layer's input; None for what is not needed.  mask: dense8.Saved.mask of a layer with a ReLU."""
+        from . import dense8
+        return dense8.linear_grad(self, dy, q, s, wq, ws, mask, need_dx, need_dw, need_db, w_dtype)
 
     # ---- measurement ------------------------------------------------------------------------
     def profile(self, on=True):

@@ -262,6 +262,61 @@ int dn_get_windows(dn_ctx *ctx, uint32_t read, uint64_t cap /* windows */, uint3
  * Parity tap: tests compare it with values the reference's own probability.cpp produced (tests/golden/ref_emission.npz). */
 int dn_debug_emission(dn_ctx *ctx, uint32_t n, const double *x, const double *mu, double *out);
 
+/* ---- 8-bit dense layers: rows of 8-bit integers with one scale each, their product, its gradient ----
+ * A dense layer over M rows (positions of reads): y = act(x W^T + b), x [M][K], W [N][K].  The network's pointwise convolutions are such
+ * layers.  Rows in 8 bits are a quarter to half of the activations' bytes and multiply at twice the 16-bit matrix rate; a layer that is
+ * being fitted keeps its input as such rows (the checkpoint) instead of numbers.  The reference has no counterpart: its network is
+ * a frozen SavedModel (tensor.cpp:12-106) and training happens outside it.
+ *   row m of x in 8 bits:  a = max_k |x|, r = 127 / a, q = rint(x r), s = a / 127, each operation rounded to fp32 (ties to even); a < 2^-120: q = 0,
+ *                          s = 0; NaN or infinity in the row: q = 0, s = NaN (the row's results are NaN)
+ *   linear:                y[m][n] = act(s[m] sw[n] sum_k q[m][k] w[n][k] + bias[n] + residual[m][n]); the sum is exact (32-bit integers)
+ *   its gradient:          dz = dy, zero where the forward pass's ReLU kept nothing (also where dy is NaN there); dx[m][k] = sum_n dz sw[n] w[n][k],
+ *                          dw[n][k] = sum_m dz s[m] q[m][k], db[n] = sum_m dz; sums in fp32, their order fixed by the sizes (the same bits every time)
+ * Unlike the stages above these calls work on the CALLER's device memory (plain pointers of the context's device, rows at a pitch of ld elements),
+ * are enqueued on the caller's stream (hip_stream: a hipStream_t, NULL = the default stream) and keep nothing: no allocation, no
+ * synchronisation, no state in the context but the error text, so they can be captured into a graph and run on several streams at once.
+ * The workspace belongs to the caller (dn_i8_*_workspace bytes, 256-byte aligned; those two calls look at the description only, ctx may be NULL) and must
+ * not be shared by calls that can overlap.  Outputs must not
+ * overlap inputs or each other.  M may be 0; 1 <= N, K <= DN_I8_MAX_K; 0 <= M < DN_I8_MAX_M.  Rows at a multiple of 16 bytes
+ * (what dn_i8_rows' callers are advised to choose) are read directly, others through the workspace. */
+enum { DN_T_F32 = 0, DN_T_F16 = 1, DN_T_BF16 = 2, DN_T_I8 = 3 };
+#define DN_I8_MAX_K 131071               /* 128 * 128 * K stays below 2^31 */
+#define DN_I8_MAX_M 2147483136ll
+/* rows of x (x_type DN_T_F32 / F16 / BF16) -> q, s.  ldq >= k; the bytes of q behind k up to the next multiple of 16 (or ldq, if that is nearer) become 0. */
+int dn_i8_rows(dn_ctx *ctx, int64_t m, int64_t k, const void *x, int64_t ldx, int x_type, int8_t *q, int64_t ldq, float *s, void *hip_stream);
+/* q s -> x, rounded once to x_type */
+int dn_i8_restore(dn_ctx *ctx, int64_t m, int64_t k, const int8_t *q, int64_t ldq, const float *s, void *x, int64_t ldx, int x_type, void *hip_stream);
+typedef struct {
+    int64_t m, n, k;
+    const void *x; int64_t ldx;         /* [m][k] of x_type */
+    const float *sx;                    /* [m], the rows' scales: given exactly if x_type is DN_T_I8 */
+    const int8_t *w; int64_t ldw;       /* [n][k] */
+    const float *sw;                    /* [n] */
+    const float *bias;                  /* [n] or NULL */
+    const void *residual; int64_t ldr;  /* [m][n] of y_type or NULL */
+    void *y; int64_t ldy;               /* [m][n] of y_type */
+    uint8_t *mask; int64_t ldmask;      /* NULL, or (with relu) one bit per output that is > 0 before rounding: bit n % 8 of byte n / 8, ldmask >= (n + 7) / 8 */
+    int8_t *q; int64_t ldq; float *s;   /* NULL, or (x not in 8 bits) the rows that were multiplied, as dn_i8_rows writes them */
+    int32_t x_type, y_type, relu, reserved;
+} dn_i8_linear_desc;
+int dn_i8_linear_workspace(dn_ctx *ctx, const dn_i8_linear_desc *d, uint64_t *bytes);
+int dn_i8_linear(dn_ctx *ctx, const dn_i8_linear_desc *d, void *workspace, uint64_t workspace_bytes, void *hip_stream);
+typedef struct {
+    int64_t m, n, k;
+    const void *dy; int64_t ldy;        /* [m][n] of dy_type */
+    const uint8_t *mask; int64_t ldmask;/* as dn_i8_linear wrote it, or NULL */
+    const int8_t *q; int64_t ldq;       /* [m][k], the checkpoint of x */
+    const float *s;                     /* [m] */
+    const int8_t *w; int64_t ldw;       /* [n][k] */
+    const float *sw;                    /* [n] */
+    void *dx; int64_t ldx;              /* [m][k] of dy_type, or NULL */
+    void *dw; int64_t lddw;             /* [n][k] of dw_type, or NULL */
+    void *db;                           /* [n] of dw_type, or NULL */
+    int32_t dy_type, dw_type;
+} dn_i8_grad_desc;
+int dn_i8_linear_grad_workspace(dn_ctx *ctx, const dn_i8_grad_desc *d, uint64_t *bytes);
+int dn_i8_linear_grad(dn_ctx *ctx, const dn_i8_grad_desc *d, void *workspace, uint64_t workspace_bytes, void *hip_stream);
+
 /* ---- measurement ---- */
 enum { DN_K_SCAN = 0, DN_K_TSTAT, DN_K_DETECT, DN_K_EVENTS, DN_K_RANKS, DN_K_QUANTILE, DN_K_PREP, DN_K_BAND_FILL,
        DN_K_BAND_TRACE, DN_K_THEILSEN, DN_K_VITERBI, DN_K_CNN /* the whole network of a batch */, DN_K_HMM, DN_K_COUNT };
