@@ -2,6 +2,7 @@
 #pragma once
 #include "dnascent_hip.h"
 #include <hip/hip_runtime.h>
+#include <algorithm>
 
 // every launcher returns hipGetLastError() of its launches; sizes, types and pointers are checked by the C entries
 hipError_t k8_rows(int64_t m, int64_t k, const void *x, int64_t ldx, int x_type, int8_t *q, int64_t ldq, float *s, hipStream_t st);

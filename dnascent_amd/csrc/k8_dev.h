@@ -1,0 +1,33 @@
+// k8_dev.h -- device helpers of the 8-bit dense layers.
+#pragma once
+#include "k8_gemm.h"
+
+typedef __bf16 k8_bf16;
+constexpr uint64_t k8_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+constexpr int K8_CUS = 256;      // compute units of an MI355X: what a launch is sized for
+
+// N values of T, 16 bytes or fewer, on T's own boundary: the memory system takes wide accesses at any address
+template <class T, int N> struct __attribute__((packed, aligned(sizeof(T)))) K8Vec { T v[N]; };
+template <class T, int N> __device__ __forceinline__ K8Vec<T, N> k8_load(const T *p) { return *(const K8Vec<T, N> *)p; }
+template <class T, int N> __device__ __forceinline__ void k8_store(T *p, const K8Vec<T, N> &v) { *(K8Vec<T, N> *)p = v; }
+
+// the largest magnitude of a row, as the bit pattern of |x|: integers order like the magnitudes, and NaN and infinity sort above every number
+__device__ __forceinline__ unsigned k8_mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+struct K8Scale { float r, s; };
+__device__ __forceinline__ K8Scale k8_scale(unsigned top) {
+    const float a = __uint_as_float(top);
+    if (top >= 0x7f800000u) return { 0.0f, __uint_as_float(0x7fc00000u) };
+    if (a < 0x1p-120f) return { 0.0f, 0.0f };
+    return { 127.0f / a, a / 127.0f };
+}
+// rint(x r) as a byte.  Adding 1.5 2^23 leaves the rounded integer (to even) in the low mantissa bits, in two's complement; |x r| < 128.
+// A row without a scale (r = 0) stores zeros whatever it holds
+__device__ __forceinline__ unsigned k8_code(float x, float r) { return __float_as_uint(x * r + 12582912.0f) & 255u; }
+__device__ __forceinline__ unsigned k8_codes(float x0, float x1, float x2, float x3, float r) {
+    if (r == 0.0f) return 0u;
+    const unsigned a = __float_as_uint(x0 * r + 12582912.0f), b = __float_as_uint(x1 * r + 12582912.0f);
+    const unsigned c = __float_as_uint(x2 * r + 12582912.0f), d = __float_as_uint(x3 * r + 12582912.0f);
+    const unsigned lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+    return lo | hi << 16;
+}
+__device__ __forceinline__ float k8_relu(float v) { return v <= 0.0f ? 0.0f : v; }      // NaN stays

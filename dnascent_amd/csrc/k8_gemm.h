@@ -1,0 +1,158 @@
+// k8_gemm.h -- the matrix product under the 8-bit dense layers: C = A B^T for rows of 8-bit integers (32-bit integer sums) or of fp16 numbers (fp32
+// sums).  Both operands have the reduction along their rows, so an operand row is a run of bytes whatever its type: 16 bytes are what one lane feeds a
+// matrix instruction (16 integers or 8 fp16), 128 bytes per row and step go through LDS, and one kernel serves both.
+//
+//   tile      BM x BN results per workgroup, WGM x WGN wavefronts, each (BM / WGM) x (BN / WGN) results in 32 x 32 blocks
+//   loads     buffer loads straight into LDS, 16 bytes per lane, two stages; the next step's loads are in flight while this one multiplies.  Rows behind
+//             the matrix and bytes behind the row's end read as zeros (bounds of the buffer descriptor; an offset no buffer has)
+//   LDS       a row's eight 16-byte pieces are stored at piece ^ key(row): eight neighbouring lanes of a fragment read hit eight different pieces
+//   results   block t of a wavefront holds columns TN c + t (c = lane & 31): a lane's TN blocks are adjacent columns, and a row leaves in runs of
+//             32 TN columns instead of 32
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float k8_f32x4 __attribute__((ext_vector_type(4)));
+typedef float k8_f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 k8_f16x8 __attribute__((ext_vector_type(8)));
+
+struct G8 {
+    const char *a, *b;           // rows at pitches of lda, ldb BYTES (multiples of 16, like the addresses)
+    int64_t lda, ldb;
+    int64_t m, n;                // rows of a, rows of b
+    int kb;                      // bytes of a row that count; i8: any number, fp16: a multiple of 16 (zeros behind the numbers)
+    int planes;                  // the reduction runs over planes of a (plane_a bytes apart) against the same b
+    int64_t plane_a;
+    int splits;                  // the reduction is cut into that many runs of steps; run z of a tile is result z
+    int tiles_m, tiles_n;
+};
+
+template <bool I8> struct K8Acc { typedef i32x16 type; };
+template <> struct K8Acc<false> { typedef k8_f32x16 type; };
+
+__device__ __forceinline__ i32x16 k8_mfma32(i32x4 a, i32x4 b, i32x16 c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ k8_f32x16 k8_mfma32(i32x4 a, i32x4 b, k8_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(k8_f16x8, a), __builtin_bit_cast(k8_f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ int k8_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const char *k8_uniform(const char *p) {
+    const uint64_t v = (uint64_t)p;
+    return (const char *)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// which tile a workgroup takes.  Workgroups are dealt to the eight XCDs round-robin: XCD x takes a contiguous run of tiles, and inside the run tiles go
+// column block by column block over groups of eight row blocks, so that what an XCD works on at a time shares rows of a and of b in its own L2
+struct K8Tile { int tm, tn, z; };
+__device__ __forceinline__ K8Tile k8_tile(const G8 &g, int bid, int total) {
+    const int per = total >> 3, rest = total & 7, x = bid & 7, i = bid >> 3;
+    const int id = x * per + min(x, rest) + i;             // XCD x has per (+ 1 if x < rest) workgroups
+    const int tiles = g.tiles_m * g.tiles_n, z = id / tiles, t = id - z * tiles;
+    const int group = 8 * g.tiles_n, gi = t / group, first = gi * 8, size = min(8, g.tiles_m - first), r = t - gi * group;
+    return { first + r % size, r / size, z };
+}
+
+// The epilogue: columns(first column of a lane), row(row), store(those, row, column, run z, values of TN adjacent columns, whether the row and column exist)
+template <bool I8, int BM, int BN, int WGM, int WGN, class Epi>
+__global__ __launch_bounds__(64 * WGM * WGN) void k8_gemm(G8 g, Epi epi) {
+    constexpr int NW = WGM * WGN, TM = BM / WGM / 32, TN = BN / WGN / 32, LOADS = (BM + BN) / 8 / NW;
+    static_assert((BM + BN) % (8 * NW) == 0 && BM % (8 * NW) == 0, "whole loads per wavefront, each of one operand");
+    __shared__ __align__(1024) char l0[(BM + BN) * 128];
+    __shared__ __align__(1024) char l1[(BM + BN) * 128];
+    typedef typename K8Acc<I8>::type acc_t;
+    const int lane = threadIdx.x & 63, wave = k8_uniform(threadIdx.x >> 6), wm = wave / WGN, wn = wave % WGN;
+    const K8Tile t = k8_tile(g, blockIdx.x, gridDim.x);
+    const int64_t m0 = (int64_t)t.tm * BM, n0 = (int64_t)t.tn * BN;
+    const int rows_a = (int)min((int64_t)BM, g.m - m0), rows_b = (int)min((int64_t)BN, g.n - n0);
+    // bytes of a tile's rows that may be read: whole 16-byte pieces up to the one with the last row's last counted byte (it cannot cross a page)
+    const unsigned na = (unsigned)((int64_t)(rows_a - 1) * g.lda + ((g.kb + 15) & ~15)), nb = (unsigned)((int64_t)(rows_b - 1) * g.ldb + ((g.kb + 15) & ~15));
+    const char *pa = k8_uniform(g.a + m0 * g.lda), *pb = k8_uniform(g.b + n0 * g.ldb);
+    const int per_plane = (g.kb + 127) >> 7, steps = per_plane * g.planes;
+    const int s0 = (int)((int64_t)steps * t.z / g.splits), s1 = (int)((int64_t)steps * (t.z + 1) / g.splits);
+    // Load i of a wavefront covers rows 8 (i NW + wave) .. + 7 of the stage, first a's, then b's.  The lane's row and piece (the one that belongs at the LDS place
+    // it writes) are the same in every load of an operand: only the buffer's base moves, and with it how many bytes of the tile are left
+    const int row8 = wave * 8 + (lane >> 3);
+    const int piece_a = ((lane & 7) ^ (row8 & 7)) * 16, piece_b = ((lane & 7) ^ ((row8 / TN) & 7)) * 16;
+    static_assert((8 * NW / TN) % 8 == 0, "b's piece does not depend on the load");
+    const unsigned off_a = (unsigned)(row8 * g.lda) + piece_a, off_b = (unsigned)(row8 * g.ldb) + piece_b;
+    auto fetch = [&](char *l, int s) {
+        const int plane = s / per_plane, k = (s - plane * per_plane) << 7;
+        const unsigned oa = k + piece_a < g.kb ? off_a + (unsigned)k : 0x80000000u, ob = k + piece_b < g.kb ? off_b + (unsigned)k : 0x80000000u;
+        const char *at = k8_uniform(pa + plane * g.plane_a);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const bool is_a = i * NW * 8 < BM;
+            const unsigned skip = (unsigned)((is_a ? i : i - BM / 8 / NW) * NW * 8) * (unsigned)(is_a ? g.lda : g.ldb), have = is_a ? na : nb;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)((is_a ? at : pb) + skip), 0, have > skip ? have - skip : 0u, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(l + (i * NW + wave) * 1024), 16, is_a ? oa : ob, 0, 0, 0);
+        }
+    };
+    acc_t acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int q = 0; q < 16; q++) acc[i][j][q] = 0;
+    const int c = lane & 31, h = lane >> 5;
+    const int abase = (wm * TM * 32 + c) * 128, akey = c & 7;
+    const int bbase = (BM + wn * TN * 32 + c * TN) * 128, bkey = c & 7;
+    auto multiply = [&](const char *l, int s) {
+        const int k = (s % per_plane) << 7;
+        const bool tail = I8 && k + 128 > g.kb;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            i32x4 a[TM], b[TN];
+            const int p = 2 * q + h;
+#pragma unroll
+            for (int i = 0; i < TM; i++) a[i] = *(const i32x4 *)(l + abase + i * 32 * 128 + ((p ^ akey) << 4));
+#pragma unroll
+            for (int j = 0; j < TN; j++) b[j] = *(const i32x4 *)(l + bbase + j * 128 + ((p ^ bkey) << 4));
+            if (tail) {                                    // integers behind the row's end: whatever is there counts as zero in one operand, which is enough
+                const int left = g.kb - k - p * 16;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int keep = left - 4 * e;
+                    const int mask = keep >= 4 ? -1 : keep <= 0 ? 0 : (1 << (8 * keep)) - 1;
+#pragma unroll
+                    for (int i = 0; i < TM; i++) a[i][e] &= mask;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+#pragma unroll
+                for (int j = 0; j < TN; j++) acc[i][j] = k8_mfma32(a[i], b[j], acc[i][j]);
+        }
+    };
+    if (s0 < s1) fetch(l0, s0);
+    int s = s0;
+    for (; s + 1 < s1; s += 2) {
+        __syncthreads();                                   // this step's loads have landed, and nobody reads the other stage any more
+        fetch(l1, s + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(l0, s);
+        __syncthreads();
+        if (s + 2 < s1) fetch(l0, s + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(l1, s + 1);
+    }
+    if (s < s1) {
+        __syncthreads();
+        multiply(l0, s);
+    }
+    // D: column lane & 31, row (q & 3) + 8 (q >> 2) + 4 h.  Lanes outside the matrix stay: an epilogue may put lanes' results together
+    const int64_t nn = n0 + wn * TN * 32 + c * TN;
+    const auto cols = epi.template columns<TN>(nn);
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int q = 0; q < 16; q++) {
+            const int64_t mm = m0 + wm * TM * 32 + i * 32 + (q & 3) + 8 * (q >> 2) + 4 * h;
+            typename Epi::value v[TN];
+#pragma unroll
+            for (int j = 0; j < TN; j++) v[j] = acc[i][j][q];
+            epi.template store<TN>(cols, epi.row(min(mm, g.m - 1)), mm, nn, t.z, v, mm < g.m && nn < g.n);
+            if (q % 4 == 3) __builtin_amdgcn_sched_barrier(0);                // a few rows at a time: the registers are full
+        }
+}
