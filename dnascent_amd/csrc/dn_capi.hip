@@ -1787,7 +1787,7 @@ static unsigned t_bytes(int t) { return t == DN_T_F32 ? 4u : t == DN_T_I8 ? 1u :
 static bool t_matrix(const void *p, int64_t rows, int64_t cols, int64_t ld, unsigned bytes, bool output) {
     if (rows == 0) return true;
     if (!p || (uintptr_t)p % bytes) return false;
-    if (ld < 0 || ld >= (1ll << 31)) return false;
+    if (ld < 0 || ld > DN_I8_MAX_PITCH / (int64_t)bytes) return false;             // the kernels' offsets inside a tile of 256 rows are 32-bit
     return ld >= cols || (rows == 1 && !output) || (!output && ld == 0);
 }
 static int i8_sizes(dn_ctx *c, const char *what, int64_t m, int64_t n, int64_t k) {
@@ -1799,7 +1799,7 @@ static int i8_sizes(dn_ctx *c, const char *what, int64_t m, int64_t n, int64_t k
     DeviceScope scope((c)->device);                                                                                        \
     if (scope.e != hipSuccess) return fail((c), DN_ERR_HIP, "hipSetDevice(%d): %s", (c)->device, hipGetErrorString(scope.e))
 #define I8_MATRIX(what, name, p, rows, cols, ld, bytes, output)                                                            \
-    if (!t_matrix((p), (rows), (cols), (ld), (bytes), (output))) return fail(c, DN_ERR_ARG, "%s: %s is missing, misaligned or has too short a pitch", what, name)
+    if (!t_matrix((p), (rows), (cols), (ld), (bytes), (output))) return fail(c, DN_ERR_ARG, "%s: %s is missing, misaligned or has a pitch that is too short or too long", what, name)
 
 int dn_i8_rows(dn_ctx *c, int64_t m, int64_t k, const void *x, int64_t ldx, int x_type, int8_t *q, int64_t ldq, float *s, void *hip_stream) {
     if (!c) return DN_ERR_ARG;

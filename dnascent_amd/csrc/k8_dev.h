@@ -11,6 +11,32 @@ template <class T, int N> struct __attribute__((packed, aligned(sizeof(T)))) K8V
 template <class T, int N> __device__ __forceinline__ K8Vec<T, N> k8_load(const T *p) { return *(const K8Vec<T, N> *)p; }
 template <class T, int N> __device__ __forceinline__ void k8_store(T *p, const K8Vec<T, N> &v) { *(K8Vec<T, N> *)p = v; }
 
+// N numbers of T as the dwords they lie in: 16-bit numbers stay two to a register
+template <class T, int N> struct K8Raw {
+    unsigned w[N * sizeof(T) / 4];
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+        else if constexpr (__is_same(T, k8_bf16)) return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+        else { typedef _Float16 h2 __attribute__((ext_vector_type(2))); return (float)__builtin_bit_cast(h2, w[e / 2])[e & 1]; }
+    }
+    __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(w, (const K8Vec<T, N> *)p, sizeof w); }
+    __device__ __forceinline__ void load(const T *p, int have) {             // the first `have`, zeros behind them
+#pragma unroll
+        for (unsigned i = 0; i < sizeof w / 4; i++) w[i] = 0u;
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (e < have) {
+                if constexpr (sizeof(T) == 4) w[e] = *(const unsigned *)(p + e);
+                else w[e / 2] |= (unsigned)*(const uint16_t *)(p + e) << (16 * (e & 1));
+            }
+    }
+    // the compiler knows nothing of what it computed from these registers before: it forms the values again instead of keeping them
+    __device__ __forceinline__ void opaque() {
+#pragma unroll
+        for (unsigned i = 0; i < sizeof w / 4; i++) asm volatile("" : "+v"(w[i]));
+    }
+};
+
 // the largest magnitude of a row, as the bit pattern of |x|: integers order like the magnitudes, and NaN and infinity sort above every number
 __device__ __forceinline__ unsigned k8_mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 struct K8Scale { float r, s; };

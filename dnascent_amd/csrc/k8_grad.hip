@@ -1,51 +1,703 @@
 // k8_grad.hip -- the gradient of the 8-bit dense layers (include/dnascent_hip.h has the formulas).
+//
+// Both products have a whole-number operand (codes, exact in fp16) and one that carries the scales: dz sw[n] for dx, dz s[m] for dw.  That one is held in fp16
+// under a power of two of its own -- per row for dx, per output channel for dw: whatever is the same for a whole sum -- which leaves it 11 bits (half a step:
+// 2^-12 of the value, for everything within 2^-24 of the row's or channel's largest; smaller values keep an absolute 2^-36 of that).  16-bit results take one such
+// piece (their own rounding is 2^-9 or 2^-12), fp32 results two (2^-23).  Sums are fp32; their order depends on the sizes alone.
 #include "k8_dense.h"
 #include "k8_dev.h"
+#include <type_traits>
 
 namespace {
 
-template <class T> __device__ __forceinline__ float k8_f32(T v) { return (float)v; }
-template <class T> __device__ __forceinline__ T k8_to(float v) { return (T)v; }
-__device__ __forceinline__ bool k8_bit(const uint8_t *mask, int64_t ld, int64_t m, int n) { return !mask || (mask[m * ld + (n >> 3)] >> (n & 7) & 1); }
+typedef _Float16 k8_f16x2 __attribute__((ext_vector_type(2)));
 
-template <class T>
-__global__ __launch_bounds__(256) void k8_dx_k(dn_i8_grad_desc d) {
-    const int64_t kb = (d.k + 255) / 256, row = blockIdx.x / kb;
-    const int k = (int)(blockIdx.x % kb) * 256 + threadIdx.x;
-    if (k >= d.k) return;
-    float acc = 0.0f;
-    for (int n = 0; n < d.n; n++)
-        if (k8_bit(d.mask, d.ldmask, row, n)) acc += k8_f32(((const T *)d.dy)[row * d.ldy + n]) * d.sw[n] * (float)d.w[(int64_t)n * d.ldw + k];
-    ((T *)d.dx)[row * d.ldx + k] = k8_to<T>(acc);
+__device__ __forceinline__ k8_f32x4 k8_mfma16(i32x4 a, i32x4 b, k8_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(k8_f16x8, a), __builtin_bit_cast(k8_f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ int k8_pack(float a, float b) { return __builtin_bit_cast(int, k8_f16x2{ (_Float16)a, (_Float16)b }); }
+// two numbers as two fp16 pieces each.  `hi` is hidden from the compiler: left to itself it forms the fp16 value that is subtracted with an instruction that rounds
+// the product behind v once, and stores the one that rounds twice.  Behind infinity and NaN there is nothing to add
+struct K8Split { int hi, lo; };
+__device__ __forceinline__ K8Split k8_split(float v0, float v1) {
+    int hi = k8_pack(v0, v1);
+    asm volatile("" : "+v"(hi));
+    const k8_f16x2 h = __builtin_bit_cast(k8_f16x2, hi);
+    const float l0 = v0 - (float)h[0], l1 = v1 - (float)h[1];
+    return { hi, k8_pack(l0 == l0 ? l0 : 0.0f, l1 == l1 ? l1 : 0.0f) };
+}
+// eight rows of four codes -> four columns of eight fp16: bytes j of two rows side by side, 0x6400 | (code ^ 0x80) is 1152 + code
+__device__ __forceinline__ void k8_columns(const unsigned (&d)[8], i32x4 (&out)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const unsigned t = __builtin_amdgcn_perm(d[2 * p + 1], d[2 * p], 0x0c000c00u | (unsigned)j | (unsigned)(4 + j) << 16) ^ 0x64806480u;
+            out[j][p] = __builtin_bit_cast(int, __builtin_bit_cast(k8_f16x2, t) - k8_f16x2{ (_Float16)1152.0f, (_Float16)1152.0f });
+        }
+}
+// the power of two that puts `top` (bits of a magnitude, finite) into [2^14, 2^15), and its inverse; both are normal numbers
+struct K8Pow { float up, down; };
+__device__ __forceinline__ K8Pow k8_pow(unsigned top) {
+    const int e = min(max(268 - (int)(top >> 23), 1), 253);
+    return { __uint_as_float((unsigned)e << 23), __uint_as_float((unsigned)(254 - e) << 23) };
 }
 
-template <class T, class W>
-__global__ __launch_bounds__(256) void k8_dw_k(dn_i8_grad_desc d) {
-    const int64_t kb = (d.k + 255) / 256;
-    const int n = (int)(blockIdx.x / kb), k = (int)(blockIdx.x % kb) * 256 + threadIdx.x;
-    float acc = 0.0f, sum = 0.0f;
-    for (int64_t m = 0; m < d.m; m++)
-        {
-            const float g = k8_bit(d.mask, d.ldmask, m, n) ? k8_f32(((const T *)d.dy)[m * d.ldy + n]) : 0.0f;
-            sum += g;
-            if (k < d.k) acc += g * d.s[m] * (float)d.q[m * d.ldq + k];
+// ---- dx, narrow layers (N <= 256) ------------------------------------------------------------------------------------------------------------------------------
+// The same shape as the forward pass over narrow rows (k8_narrow): a wavefront takes MT x 16 rows of dy, holds them in registers in the matrix operand's order,
+// finds each row's power of two, and multiplies with the weight, whose transposed fragments lie in LDS as fp16 (256 k x N).  Nothing but dy, the mask and dx
+// moves.  NP: pieces.
+template <class T, int NS, int MT, int NP>
+__global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d) {
+    __shared__ __align__(16) char lw[256 * NS * 64];       // fragment (k block of 64, tile t, step) x 64 lanes x 16 bytes: column k = 64 blk + 4 c + t, n = 32 step + 8 g ..
+    __shared__ __align__(16) float lsw[NS * 32];
+    const int lane = threadIdx.x & 63, wave = k8_uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const int n = (int)d.n;
+    const int64_t k0 = (int64_t)blockIdx.y * 256;
+    const int cols = (int)min((int64_t)256, d.k - k0), blocks = (cols + 63) / 64;
+    for (int f = threadIdx.x; f < blocks * NS * 64; f += 512) {
+        const int fc = f & 15, fg = (f >> 4) & 3, step = (f >> 6) % NS, blk = (f >> 6) / NS, kk = blk * 64 + 4 * fc;
+        unsigned rows[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int nn = step * 32 + 8 * fg + e;
+            rows[e] = 0;
+            if (nn < n) {
+                const int8_t *wr = d.w + nn * d.ldw + k0 + kk;
+                if (kk + 4 <= cols) __builtin_memcpy(&rows[e], wr, 4);
+                else
+                    for (int b = 0; b < 4; b++) if (kk + b < cols) rows[e] |= (unsigned)(uint8_t)wr[b] << (8 * b);
+            }
         }
-    if (d.dw && k < d.k) ((W *)d.dw)[n * d.lddw + k] = k8_to<W>(acc);
-    if (d.db && k == 0) ((W *)d.db)[n] = k8_to<W>(sum);
+        i32x4 out[4];
+        k8_columns(rows, out);
+#pragma unroll
+        for (int t = 0; t < 4; t++) *(i32x4 *)(lw + (((blk * 4 + t) * NS + step) * 64 + fg * 16 + fc) * 16) = out[t];
+    }
+    for (int i = threadIdx.x; i < NS * 32; i += 512) lsw[i] = i < n ? d.sw[i] : 0.0f;
+    __syncthreads();
+    const int64_t tiles = (d.m + 16 * MT - 1) / (16 * MT), stride = (int64_t)gridDim.x * 8;
+    K8Raw<T, 8> raw[MT][NS];
+    unsigned bit[MT][NS];
+    auto fetch = [&](int64_t tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            const int64_t row = min((tile * MT + i) * 16 + c, d.m - 1);
+            const T *p = (const T *)d.dy + row * d.ldy;
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const int at = s * 32 + 8 * g;
+                if (at + 8 <= n) raw[i][s].load(p + at);
+                else raw[i][s].load(p + at, n - at);
+                bit[i][s] = d.mask && at < n ? d.mask[row * d.ldmask + (at >> 3)] : 255u;
+            }
+        }
+    };
+    int64_t tile = (int64_t)blockIdx.x * 8 + wave;
+    if (tile < tiles) fetch(tile);
+    for (; tile < tiles; tile += stride) {
+        i32x4 a[MT][NP][NS];
+        float down[MT];
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            // the row's largest dz sw, then the pieces under its power of two.  (dz sw is formed twice: the products are cheaper than the registers.)
+            auto value = [&](int s, int e, const K8Vec<float, 8> &sw) { return (bit[i][s] >> e & 1 ? raw[i][s].get(e) : 0.0f) * sw.v[e]; };
+            unsigned top = 0;
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = max(top, k8_mag(value(s, e, sw)));
+            }
+            top = max(top, (unsigned)__shfl_xor((int)top, 16));
+            top = max(top, (unsigned)__shfl_xor((int)top, 32));
+            if (__any(top >= 0x7f800000u)) {               // not finite: the others' power of two is taken from the finite ones
+                top = 0;
+#pragma unroll
+                for (int s = 0; s < NS; s++) {
+                    const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + 8 * g);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) { const unsigned v = k8_mag(value(s, e, sw)); top = max(top, v < 0x7f800000u ? v : 0u); }
+                }
+                top = max(top, (unsigned)__shfl_xor((int)top, 16));
+                top = max(top, (unsigned)__shfl_xor((int)top, 32));
+            }
+            const K8Pow pw = k8_pow(top);
+            down[i] = pw.down;
+            // the second pass forms the products again from these registers: 64 of them kept as fp32 do not fit beside the rest
+#pragma unroll
+            for (int s = 0; s < NS; s++) raw[i][s].opaque();
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + 8 * g);
+#pragma unroll
+                for (int p = 0; p < 4; p++) {
+                    const float v0 = value(s, 2 * p, sw) * pw.up, v1 = value(s, 2 * p + 1, sw) * pw.up;
+                    if (NP == 2) {
+                        const K8Split w = k8_split(v0, v1);
+                        a[i][0][s][p] = w.hi; a[i][NP - 1][s][p] = w.lo;
+                    } else a[i][0][s][p] = k8_pack(v0, v1);
+                }
+            }
+        }
+        if (tile + stride < tiles) fetch(tile + stride);
+        float rs[MT][4];
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) rs[i][q] = __shfl(down[i], 4 * g + q);
+        for (int blk = 0; blk < blocks; blk++) {
+            k8_f32x4 acc[MT][4];
+            const char *lb = lw + (blk * 4 * NS * 64 + lane) * 16;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+#pragma unroll
+                for (int i = 0; i < MT; i++) acc[i][t] = k8_f32x4{ 0, 0, 0, 0 };
+#pragma unroll
+                for (int s = 0; s < NS; s++) {
+                    const i32x4 b = *(const i32x4 *)(lb + (t * NS + s) * 1024);
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int p = 0; p < NP; p++) acc[i][t] = k8_mfma16(a[i][p][s], b, acc[i][t]);
+                }
+            }
+            const int64_t kk = k0 + blk * 64 + 4 * c;
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int64_t mm = (tile * MT + i) * 16 + 4 * g + q;
+                    if (mm >= d.m || kk >= d.k) continue;
+                    T *p = (T *)d.dx + mm * d.ldx + kk;
+                    K8Vec<T, 4> o;
+#pragma unroll
+                    for (int t = 0; t < 4; t++) o.v[t] = (T)(acc[i][t][q] * rs[i][q]);
+                    if (kk + 4 <= d.k) k8_store<T, 4>(p, o);
+                    else
+#pragma unroll
+                        for (int t = 0; t < 4; t++) if (kk + t < d.k) p[t] = o.v[t];
+                }
+        }
+    }
+}
+
+// ---- dx, wide layers: the pieces of dz sw as rows of fp16, the transposed weight as rows of fp16, then k8_gemm -----------------------------------------------------
+// LPR lanes walk a row twice (the second time from cache).  np: pitch in fp16, a multiple of 8; zeros behind n
+template <class T, int LPR, int NP>
+__global__ __launch_bounds__(256) void k8_pieces(dn_i8_grad_desc d, _Float16 *__restrict__ out, int np, int64_t plane, float *__restrict__ down) {
+    const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    const int lid = threadIdx.x % LPR, n = (int)d.n;
+    const int64_t rr = min(row, d.m - 1);
+    const T *p = (const T *)d.dy + rr * d.ldy;
+    const uint8_t *mk = d.mask ? d.mask + rr * d.ldmask : nullptr;
+    float v[8];
+    auto piece = [&](int at) {
+        const unsigned bits = mk ? mk[at >> 3] : 255u;
+        K8Vec<T, 8> x; K8Vec<float, 8> sw;
+        if (at + 8 <= n) { x = k8_load<T, 8>(p + at); sw = k8_load<float, 8>(d.sw + at); }
+        else
+#pragma unroll
+            for (int e = 0; e < 8; e++) { x.v[e] = at + e < n ? p[at + e] : (T)0.0f; sw.v[e] = at + e < n ? d.sw[at + e] : 0.0f; }
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = (bits >> e & 1 ? (float)x.v[e] : 0.0f) * sw.v[e];
+    };
+    unsigned top = 0;
+    for (int at = lid * 8; at < n; at += LPR * 8) {
+        piece(at);
+#pragma unroll
+        for (int e = 0; e < 8; e++) { const unsigned b = k8_mag(v[e]); top = max(top, b < 0x7f800000u ? b : 0u); }
+    }
+#pragma unroll
+    for (int o = (LPR < 64 ? LPR : 64) / 2; o; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
+    if (LPR == 256) {
+        __shared__ unsigned part[4];
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+        __syncthreads();
+        top = max(max(part[0], part[1]), max(part[2], part[3]));
+    }
+    if (row >= d.m) return;
+    const K8Pow pw = k8_pow(top);
+    if (lid == 0) down[row] = pw.down;
+    for (int at = lid * 8; at < np; at += LPR * 8) {
+        i32x4 hi, lo;
+        if (at < n) piece(at);
+        else
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const K8Split w = k8_split(v[2 * q] * pw.up, v[2 * q + 1] * pw.up);
+            hi[q] = w.hi; lo[q] = w.lo;
+        }
+        *(i32x4 *)(out + row * np + at) = hi;
+        if (NP == 2) *(i32x4 *)(out + plane + row * np + at) = lo;
+    }
+}
+// w [n][k] codes -> [k][np] fp16, zeros behind n.  A thread takes 8 n x 4 k; the 8 lanes beside it the next 64 n
+__global__ __launch_bounds__(256) void k8_turn(dn_i8_grad_desc d, _Float16 *__restrict__ out, int np) {
+    const int n = (int)d.n, k = (int)d.k;
+    const int64_t nb = (np + 63) / 64, kb = (k + 127) / 128;
+    const int64_t bn = blockIdx.x % nb, bk = blockIdx.x / nb;
+    if (bk >= kb) return;
+    const int nn = (int)bn * 64 + (threadIdx.x & 7) * 8, kk = (int)bk * 128 + (threadIdx.x >> 3) * 4;
+    if (nn >= np || kk >= k) return;
+    unsigned rows[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        rows[e] = 0;
+        if (nn + e < n) {
+            const int8_t *wr = d.w + (int64_t)(nn + e) * d.ldw + kk;
+            if (kk + 4 <= k) __builtin_memcpy(&rows[e], wr, 4);
+            else
+                for (int b = 0; b < 4; b++) if (kk + b < k) rows[e] |= (unsigned)(uint8_t)wr[b] << (8 * b);
+        }
+    }
+    i32x4 o[4];
+    k8_columns(rows, o);
+#pragma unroll
+    for (int j = 0; j < 4; j++) if (kk + j < k) *(i32x4 *)(out + (int64_t)(kk + j) * np + nn) = o[j];
+}
+template <class T>
+struct DxEpi {
+    typedef float value;
+    const float *down; T *dx; int64_t k, ldx;
+    template <int TN> struct Columns {};
+    template <int TN> __device__ __forceinline__ Columns<TN> columns(int64_t) const { return {}; }
+    __device__ __forceinline__ float row(int64_t mm) const { return down[mm]; }
+    template <int TN> __device__ __forceinline__ void store(const Columns<TN> &, float s, int64_t mm, int64_t kk, int, const float (&acc)[TN], bool live) const {
+        if (!live) return;
+        T *p = dx + mm * ldx + kk;
+        K8Vec<T, TN> o;
+#pragma unroll
+        for (int j = 0; j < TN; j++) o.v[j] = (T)(acc[j] * s);
+        if (kk + TN <= k) k8_store<T, TN>(p, o);
+        else
+#pragma unroll
+            for (int j = 0; j < TN; j++) if (kk + j < k) p[j] = o.v[j];
+    }
+};
+// a run's sums: part [splits][m][k]
+struct DxPart {
+    typedef float value;
+    float *part; int64_t m, k;
+    template <int TN> struct Columns {};
+    template <int TN> __device__ __forceinline__ Columns<TN> columns(int64_t) const { return {}; }
+    __device__ __forceinline__ float row(int64_t) const { return 0.0f; }
+    template <int TN> __device__ __forceinline__ void store(const Columns<TN> &, float, int64_t mm, int64_t kk, int z, const float (&acc)[TN], bool live) const {
+        if (!live) return;
+        float *p = part + ((int64_t)z * m + mm) * k + kk;
+#pragma unroll
+        for (int j = 0; j < TN; j++) if (kk + j < k) p[j] = acc[j];
+    }
+};
+template <class T>
+__global__ __launch_bounds__(256) void k8_dx_join(const float *__restrict__ part, int splits, const float *__restrict__ down, T *__restrict__ dx, int64_t m, int64_t k, int64_t ldx) {
+    const int64_t kb = (k + 255) / 256, w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (w >= m * kb) return;
+    const int64_t mm = w / kb, kk = (w % kb) * 256 + (threadIdx.x & 63) * 4;
+    for (int j = 0; j < 4 && kk + j < k; j++) {
+        float s = 0.0f;
+        for (int z = 0; z < splits; z++) s += part[((int64_t)z * m + mm) * k + kk + j];
+        dx[mm * ldx + kk + j] = (T)(s * down[mm]);
+    }
+}
+
+// ---- dw and db --------------------------------------------------------------------------------------------------------------------------------------------------
+// The reduction runs over rows, along which neither operand is contiguous.  A workgroup takes S x S results (output channels x input channels) and a run of rows,
+// RT at a time: a thread reads eight rows of four adjacent channels, makes the fp16 values and writes them to LDS turned -- eight rows of one channel are the
+// 16 bytes a matrix instruction takes.  The rows of the next tile are in flight while this one multiplies.
+//
+// Every output channel has a power of two, agreed on by the whole workgroup: it starts so high that the first number which is not tiny does not fit, and whoever
+// sees one that does not fit raises a flag; behind the barrier the workgroup then finds the tile's largest numbers, lowers the powers of the channels that need
+// it (five bits of room), scales their sums so far -- exactly -- and makes the tile again.  That happens for a workgroup's first tile and hardly ever after.
+//
+// LDS row of a channel: RT rows x 2 bytes (x NP pieces), in pieces of 16 bytes at piece ^ ((channel >> 2) & 7): threads that write and lanes that read four channels
+// apart hit different banks.  Wavefronts share the S x S results in blocks of 64 x KB; where there are fewer blocks than wavefronts, sets of wavefronts take turns
+// with the steps of 32 rows and join their sums at the end.
+template <int S, int NP> struct DwShape {
+    static constexpr int RT = 16384 / S / NP;              // rows of a tile: S = 256: 64, 128: 128, 64: 256 (half with two pieces)
+    static constexpr int KB = S == 256 ? 128 : 64, BLOCKS = (S / 64) * (S / KB), SETS = 8 / BLOCKS, STEPS = RT / 32;
+    static constexpr int UROW = RT * 2 * NP, QROW = RT * 2; // bytes of a channel's row
+    static constexpr int LDS = S * (UROW + QROW);           // one stage
+};
+struct DwOut { float *part, *part_b; int splits, tiles_n, tiles_k; int64_t run; };   // part [splits][n][k], part_b [splits][n]; run: rows of a split, a multiple of RT
+
+template <class W> __device__ __forceinline__ void k8_put4(W *p, const float (&v)[4], int64_t left) {
+    K8Vec<W, 4> o;
+#pragma unroll
+    for (int j = 0; j < 4; j++) o.v[j] = (W)v[j];
+    if (left >= 4) k8_store<W, 4>(p, o);
+    else
+#pragma unroll
+        for (int j = 0; j < 4; j++) if (j < left) p[j] = o.v[j];
+}
+__device__ __forceinline__ void k8_put4(void *p, int type, int64_t at, const float (&v)[4], int64_t left) {
+    if (type == DN_T_F32) k8_put4((float *)p + at, v, left);
+    else if (type == DN_T_F16) k8_put4((_Float16 *)p + at, v, left);
+    else k8_put4((k8_bf16 *)p + at, v, left);
+}
+
+template <class T, int S, int NP>
+__global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
+    typedef DwShape<S, NP> D;
+    __shared__ __align__(1024) char lds[2][D::LDS];
+    __shared__ float power[S], lower[S];
+    __shared__ unsigned peak[S];
+    __shared__ int raised[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = k8_uniform(tid >> 6), c = lane & 15, g = lane >> 4;
+    const int tiles = o.tiles_n * o.tiles_k, z = blockIdx.x / tiles, t = blockIdx.x % tiles, tn = t % o.tiles_n, tk = t / o.tiles_n;
+    const int64_t n0 = (int64_t)tn * S, k0 = (int64_t)tk * S, r0 = (int64_t)z * o.run, r1 = min(r0 + o.run, d.m);
+    const int ncols = (int)min((int64_t)S, d.n - n0), kcols = (int)min((int64_t)S, d.k - k0);
+    const bool with_q = d.dw != nullptr, with_b = d.db != nullptr && tk == 0;
+    for (int i = tid; i < S; i += 512) power[i] = 0x1p126f;
+    if (tid < 2) raised[tid] = 0;
+    __syncthreads();
+    // a task: eight rows x four channels.  S / 4 tasks across, RT / 8 down; with RT S = 16384 / NP that is 512 / NP for each of dy and q: one per thread, or with two
+    // pieces dy's for the first four wavefronts and q's for the others
+    constexpr int ACROSS = S / 4, TASKS = ACROSS * (D::RT / 8);
+    static_assert(TASKS == 512 / NP, "one task per thread");
+    const bool has_u = tid < TASKS, has_q = NP == 1 || tid >= TASKS;
+    const int task = NP == 1 ? tid : tid & (TASKS - 1), ch = (task % ACROSS) * 4, rg = task / ACROSS;      // first channel, group of eight rows
+    K8Raw<T, 4> raw[8];
+    unsigned rq[8], rbit[8];
+    float rs[8];
+    // Row addresses are a uniform base and one 32-bit offset per lane and operand.  Rows behind the run repeat its last one and count as zeros (no mask bit, no scale)
+    const bool u_whole = ch + 4 <= ncols, q_whole = ch + 4 <= kcols, u_in = has_u && ch < ncols, q_in = has_q && with_q && ch < kcols;
+    const int esh = (int)((n0 + ch) & 7);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        rbit[e] = ch < ncols ? 255u : 0u; rs[e] = 0.0f; rq[e] = 0u;
+#pragma unroll
+        for (unsigned j = 0; j < sizeof(T); j++) raw[e].w[j] = 0u;
+    }
+    auto fetch_rows = [&](int64_t base, auto full) __attribute__((always_inline)) {
+        constexpr bool FULL = decltype(full)::value;
+        const char *pu = k8_uniform((const char *)d.dy + (base * d.ldy + n0) * (int64_t)sizeof(T)), *pq = k8_uniform((const char *)d.q + base * d.ldq + k0);
+        const char *pm = k8_uniform((const char *)d.mask + base * d.ldmask + (n0 >> 3)), *ps = k8_uniform((const char *)(d.s + base));
+        const int left = (int)min(r1 - base, (int64_t)D::RT) - 1;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            // FULL: lane offset to the group's first row, the other rows by the base; else every row by itself
+            const unsigned r = FULL ? (unsigned)(rg * 8) : (unsigned)min(rg * 8 + e, left);
+            const int64_t up = FULL ? e : 0;
+            if (u_in) {
+                if (with_q) rs[e] = *(const float *)(ps + up * 4 + r * 4u);
+                const T *p = (const T *)(pu + up * d.ldy * (int64_t)sizeof(T) + (r * (unsigned)d.ldy + (unsigned)ch) * (unsigned)sizeof(T));
+                if (u_whole) raw[e].load(p);
+                else raw[e].load(p, ncols - ch);
+                if (d.mask) rbit[e] = (unsigned)*(const uint8_t *)(pm + up * d.ldmask + r * (unsigned)d.ldmask + (unsigned)(ch >> 3)) >> esh;
+                if (!FULL && rg * 8 + e > left) { rbit[e] = 0u; rs[e] = 0.0f; }
+                else if (!FULL && !d.mask) rbit[e] = 255u;
+            }
+            if (q_in) {
+                const char *p = pq + up * d.ldq + r * (unsigned)d.ldq + (unsigned)ch;
+                if (q_whole) __builtin_memcpy(&rq[e], p, 4);
+                else {
+                    rq[e] = 0u;
+#pragma unroll
+                    for (int j = 0; j < 3; j++) if (ch + j < kcols) rq[e] |= (unsigned)*(const uint8_t *)(p + j) << (8 * j);
+                }
+            }
+        }
+    };
+    auto fetch = [&](int64_t base) __attribute__((always_inline)) {
+        if (base + D::RT <= r1) fetch_rows(base, std::true_type());
+        else fetch_rows(base, std::false_type());
+    };
+    float pw[4] = { 0x1p126f, 0x1p126f, 0x1p126f, 0x1p126f }, sum[4] = { 0, 0, 0, 0 };
+    auto dz = [&](int e, int j) { return rbit[e] >> j & 1 ? raw[e].get(j) : 0.0f; };
+    // the turned fp16 values of this thread's task (and, the first time, the sums of dz); true if one does not fit
+    auto make = [&](char *l, auto first) __attribute__((always_inline)) {
+        float most = 0.0f;
+        if (has_u)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                i32x4 hi, lo;
+#pragma unroll
+                for (int p = 0; p < 4; p++) {
+                    const float z0 = dz(2 * p, j), z1 = dz(2 * p + 1, j), v0 = z0 * rs[2 * p] * pw[j], v1 = z1 * rs[2 * p + 1] * pw[j];
+                    if (decltype(first)::value) sum[j] = sum[j] + z0 + z1;
+                    most = fmaxf(most, fmaxf(fabsf(v0), fabsf(v1)));
+                    if (NP == 2) { const K8Split w = k8_split(v0, v1); hi[p] = w.hi; lo[p] = w.lo; }
+                    else hi[p] = k8_pack(v0, v1);
+                }
+                const int key = ((ch + j) >> 2) & 7;
+                char *row = l + (ch + j) * D::UROW;
+                *(i32x4 *)(row + ((rg ^ key) << 4)) = hi;
+                if (NP == 2) *(i32x4 *)(row + (((rg + D::RT / 8) ^ key) << 4)) = lo;
+            }
+        return most > 32768.0f;
+    };
+    auto make_q = [&](char *l) __attribute__((always_inline)) {
+        if (!has_q) return;
+        i32x4 out[4];
+        k8_columns(rq, out);
+#pragma unroll
+        for (int j = 0; j < 4; j++) *(i32x4 *)(l + S * D::UROW + (ch + j) * D::QROW + ((rg ^ (((ch + j) >> 2) & (D::QROW >= 128 ? 7 : 3))) << 4)) = out[j];
+    };
+    const int block = wave % D::BLOCKS, set = wave / D::BLOCKS, bn = block % (S / 64), bk = block / (S / 64);
+    constexpr int TK = D::KB / 16;
+    k8_f32x4 acc[4][TK];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < TK; j++) acc[i][j] = k8_f32x4{ 0, 0, 0, 0 };
+    // tile i of a block of 64 holds channels 4 c + i: key = c & 7
+    auto multiply = [&](const char *l) __attribute__((always_inline)) {
+#pragma unroll
+        for (int w = 0; w < (D::STEPS * NP + D::SETS - 1) / D::SETS; w++) {
+            const int item = w * D::SETS + set, step = item % D::STEPS, plane = item / D::STEPS;
+            if (D::STEPS * NP % D::SETS && item >= D::STEPS * NP) break;
+            i32x4 a[4], b[TK];
+#pragma unroll
+            for (int i = 0; i < 4; i++) a[i] = *(const i32x4 *)(l + (bn * 64 + 4 * c + i) * D::UROW + (((plane * (D::RT / 8) + step * 4 + g) ^ (c & 7)) << 4));
+#pragma unroll
+            for (int j = 0; j < TK; j++)
+                b[j] = *(const i32x4 *)(l + S * D::UROW + (bk * D::KB + (j / 4) * 64 + 4 * c + j % 4) * D::QROW + (((step * 4 + g) ^ (c & (D::QROW >= 128 ? 7 : 3))) << 4));
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < TK; j++) acc[i][j] = k8_mfma16(a[i], b[j], acc[i][j]);
+        }
+    };
+    if (r0 < r1) fetch(r0);                                // (a call without rows has one empty run: its sums are zeros)
+    int stage = 0;
+    for (int64_t base = r0; base < r1; base += D::RT, stage ^= 1) {
+        char *l = lds[stage];
+        const bool over = make(l, std::true_type());
+        if (with_q) {
+            make_q(l);
+            if (over) raised[stage] = 1;                   // (any lane; all that write write 1)
+            __syncthreads();
+            if (raised[stage]) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) raw[e].opaque();
+                for (int i = tid; i < S; i += 512) peak[i] = 0u;
+                __syncthreads();
+                if (has_u)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        unsigned top = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) { const unsigned v = k8_mag(dz(e, j) * rs[e]); top = max(top, v < 0x7f800000u ? v : 0u); }
+                        atomicMax(&peak[ch + j], top);
+                    }
+                __syncthreads();
+                for (int i = tid; i < S; i += 512) {
+                    const float was = power[i], a = __uint_as_float(peak[i]);
+                    float now = was;
+                    if (a * was > 32768.0f) now = __uint_as_float((unsigned)min(max(264 - (int)(peak[i] >> 23), 1), 253) << 23);     // a -> [2^10, 2^11)
+                    power[i] = now;
+                    lower[i] = now / was;
+                }
+                if (tid == 0) raised[stage] = 0;
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < 4; j++) pw[j] = power[ch + j];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const float f = lower[bn * 64 + 4 * (4 * g + q) + i];
+#pragma unroll
+                        for (int j = 0; j < TK; j++) acc[i][j][q] *= f;
+                    }
+#pragma unroll
+                for (int e = 0; e < 8; e++) raw[e].opaque();
+                (void)make(l, std::false_type());
+                __syncthreads();
+            }
+        }
+        if (base + D::RT < r1) fetch(base + D::RT);
+        if (with_q) multiply(l);
+    }
+    // ---- the sums leave: sets of wavefronts joined in LDS first, in the order of the sets
+    __syncthreads();
+    const bool last = o.splits == 1;
+    if (with_q) {
+        float *js = (float *)lds;                          // [blocks][4 * TK * 4][64] floats
+        if (D::SETS > 1)
+            for (int s = 1; s < D::SETS; s++) {
+                if (set == s)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int j = 0; j < TK; j++)
+                            *(k8_f32x4 *)(js + ((block * 4 + i) * TK + j) * 256 + lane * 4) = acc[i][j];
+                __syncthreads();
+                if (set == 0)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int j = 0; j < TK; j++) acc[i][j] += *(const k8_f32x4 *)(js + ((block * 4 + i) * TK + j) * 256 + lane * 4);
+                __syncthreads();
+            }
+        if (set == 0)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int cn = bn * 64 + 4 * (4 * g + q) + i;
+                    if (cn >= ncols) continue;
+                    const float f = 1.0f / power[cn];
+#pragma unroll
+                    for (int j = 0; j < TK / 4; j++) {
+                        const int ck = bk * D::KB + j * 64 + 4 * c;
+                        if (ck >= kcols) continue;
+                        const float v[4] = { acc[i][4 * j][q] * f, acc[i][4 * j + 1][q] * f, acc[i][4 * j + 2][q] * f, acc[i][4 * j + 3][q] * f };
+                        if (last) k8_put4(d.dw, d.dw_type, (n0 + cn) * d.lddw + k0 + ck, v, kcols - ck);
+                        else k8_put4(o.part + ((int64_t)z * d.n + n0 + cn) * d.k + k0 + ck, v, kcols - ck);
+                    }
+                }
+        __syncthreads();
+    }
+    if (with_b) {
+        float *js = (float *)lds;                          // [RT / 8][S]
+        if (has_u)
+#pragma unroll
+            for (int j = 0; j < 4; j++) js[rg * S + ch + j] = sum[j];
+        __syncthreads();
+        for (int i = tid; i < ncols; i += 512) {
+            float v = 0.0f;
+            for (int r = 0; r < D::RT / 8; r++) v += js[r * S + i];
+            if (!last) o.part_b[(int64_t)z * d.n + n0 + i] = v;
+            else if (d.dw_type == DN_T_F32) ((float *)d.db)[n0 + i] = v;
+            else if (d.dw_type == DN_T_F16) ((_Float16 *)d.db)[n0 + i] = (_Float16)v;
+            else ((k8_bf16 *)d.db)[n0 + i] = (k8_bf16)v;
+        }
+    }
+}
+// the runs joined: 64 lanes x four adjacent results, four wavefronts a quarter of the runs each
+__global__ __launch_bounds__(256) void k8_dw_join(const float *__restrict__ part, int splits, int64_t rows, int64_t k, void *__restrict__ out, int type, int64_t ld) {
+    __shared__ float js[4][64][4];
+    const int64_t kb = (k + 255) / 256, r = blockIdx.x / kb, kk = (blockIdx.x % kb) * 256 + (threadIdx.x & 63) * 4;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    float v[4] = { 0, 0, 0, 0 };
+    if (kk < k)
+#pragma unroll 4
+        for (int z = wave; z < splits; z += 4) {
+            const float *p = part + ((int64_t)z * rows + r) * k + kk;
+            if (kk + 4 <= k) {
+                const K8Vec<float, 4> t = k8_load<float, 4>(p);
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[j] += t.v[j];
+            } else
+#pragma unroll
+                for (int j = 0; j < 4; j++) if (kk + j < k) v[j] += p[j];
+        }
+#pragma unroll
+    for (int j = 0; j < 4; j++) js[wave][lane][j] = v[j];
+    __syncthreads();
+    if (wave == 0 && kk < k) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = js[0][lane][j] + js[1][lane][j] + js[2][lane][j] + js[3][lane][j];
+        k8_put4(out, type, r * ld + kk, v, k - kk);
+    }
+}
+
+// ---- which way a call takes.  Nothing here looks at which results are asked for: a result's bits do not depend on its company -----------------------------------------
+struct Plan {
+    bool narrow = false, big = false; int dx_splits = 1, np_x = 1, np_w = 1, pitch = 0;
+    int s = 256, tiles_n = 1, tiles_k = 1, splits = 1; int64_t run = 0;
+    uint64_t pieces = 0, turned = 0, down = 0, dx_part = 0, part = 0, part_b = 0, total = 0;
+};
+Plan plan_grad(const dn_i8_grad_desc &d) {
+    Plan p;
+    auto take = [&](uint64_t bytes) { const uint64_t at = p.total; p.total += k8_up(bytes, 256); return at; };
+    p.np_x = d.dy_type == DN_T_F32 ? 2 : 1;
+    p.np_w = d.dw_type == DN_T_F32 ? 2 : 1;
+    p.narrow = d.n <= 256 && d.k <= 512;
+    if (d.dx && d.m && !p.narrow) {
+        p.pitch = (int)k8_up(d.n, 8);
+        p.pieces = take((uint64_t)p.np_x * d.m * p.pitch * 2);
+        p.turned = take((uint64_t)d.k * p.pitch * 2);
+        p.down = take((uint64_t)d.m * 4);
+        const int64_t t256 = ((d.m + 255) / 256) * ((d.k + 255) / 256), t128 = ((d.m + 127) / 128) * ((d.k + 127) / 128), steps = (p.pitch * 2 + 127) / 128 * p.np_x;
+        p.big = t256 >= K8_CUS;
+        if (!p.big && t128 < K8_CUS) {
+            p.dx_splits = (int)std::max<int64_t>(1, std::min<int64_t>(K8_CUS / t128, steps / 4));
+            if (p.dx_splits > 1) p.dx_part = take((uint64_t)p.dx_splits * d.m * d.k * 4);
+        }
+    }
+    const int64_t widest = std::max(d.n, d.k);
+    p.s = widest <= 64 ? 64 : widest <= 128 ? 128 : 256;
+    const int64_t rt = 16384 / p.s / p.np_w, row_tiles = std::max<int64_t>(1, (d.m + rt - 1) / rt);
+    p.tiles_n = (int)((d.n + p.s - 1) / p.s); p.tiles_k = (int)((d.k + p.s - 1) / p.s);
+    const int64_t want = std::max<int64_t>(1, K8_CUS / ((int64_t)p.tiles_n * p.tiles_k)), each = (row_tiles + want - 1) / want;
+    p.run = each * rt;
+    p.splits = (int)((row_tiles + each - 1) / each);
+    if (p.splits > 1) {
+        if (d.dw) p.part = take((uint64_t)p.splits * d.n * d.k * 4);
+        if (d.db) p.part_b = take((uint64_t)p.splits * d.n * 4);
+    }
+    return p;
+}
+
+template <class T, int NP, class Epi> hipError_t dx_gemm(const dn_i8_grad_desc &d, const Plan &p, char *base, const Epi &e, hipStream_t st) {
+    const int b = p.big ? 256 : 128;
+    const int64_t plane = d.m * (int64_t)p.pitch * 2;
+    G8 g = { base + p.pieces, base + p.turned, (int64_t)p.pitch * 2, (int64_t)p.pitch * 2, d.m, d.k, p.pitch * 2, NP, plane, p.dx_splits,
+             (int)((d.m + b - 1) / b), (int)((d.k + b - 1) / b) };
+    const unsigned grid = (unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits);
+    if (p.big) k8_gemm<false, 256, 256, 2, 4, Epi><<<dim3(grid), 512, 0, st>>>(g, e);
+    else k8_gemm<false, 128, 128, 2, 2, Epi><<<dim3(grid), 256, 0, st>>>(g, e);
+    return hipGetLastError();
+}
+template <class T, int NP> hipError_t dx_of(const dn_i8_grad_desc &d, const Plan &p, char *base, hipStream_t st) {
+    if (p.narrow) {
+        constexpr int MT = NP == 1 ? 2 : 1;
+        const unsigned per = (unsigned)((d.k + 255) / 256);
+        const int64_t wgs = (d.m + 128 * MT - 1) / (128 * MT);
+        if (d.n <= 64) k8_dx_narrow<T, 2, MT, NP><<<dim3((unsigned)std::min<int64_t>(wgs, 2 * K8_CUS / per), per), 512, 0, st>>>(d);
+        else if (d.n <= 128) k8_dx_narrow<T, 4, MT, NP><<<dim3((unsigned)std::min<int64_t>(wgs, 2 * K8_CUS / per), per), 512, 0, st>>>(d);
+        else k8_dx_narrow<T, 8, MT, NP><<<dim3((unsigned)std::min<int64_t>(wgs, K8_CUS / per), per), 512, 0, st>>>(d);
+        return hipGetLastError();
+    }
+    _Float16 *pieces = (_Float16 *)(base + p.pieces), *turned = (_Float16 *)(base + p.turned);
+    float *down = (float *)(base + p.down);
+    const int64_t plane = d.m * (int64_t)p.pitch;
+    if (d.n <= 2048 && d.m >= 4 * K8_CUS) k8_pieces<T, 64, NP><<<dim3((unsigned)((d.m + 3) / 4)), 256, 0, st>>>(d, pieces, p.pitch, plane, down);
+    else k8_pieces<T, 256, NP><<<dim3((unsigned)d.m), 256, 0, st>>>(d, pieces, p.pitch, plane, down);
+    k8_turn<<<dim3((unsigned)(((p.pitch + 63) / 64) * ((d.k + 127) / 128))), 256, 0, st>>>(d, turned, p.pitch);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (p.dx_splits == 1) return dx_gemm<T, NP>(d, p, base, DxEpi<T>{ down, (T *)d.dx, d.k, d.ldx }, st);
+    const DxPart part = { (float *)(base + p.dx_part), d.m, d.k };
+    e = dx_gemm<T, NP>(d, p, base, part, st);
+    if (e != hipSuccess) return e;
+    k8_dx_join<T><<<dim3((unsigned)((d.m * ((d.k + 255) / 256) + 3) / 4)), 256, 0, st>>>(part.part, p.dx_splits, down, (T *)d.dx, d.m, d.k, d.ldx);
+    return hipGetLastError();
+}
+template <class T, int NP> hipError_t dw_of(const dn_i8_grad_desc &d, const Plan &p, char *base, hipStream_t st) {
+    const int tiles_k = d.dw ? p.tiles_k : 1;
+    const DwOut o = { (float *)(base + p.part), (float *)(base + p.part_b), p.splits, p.tiles_n, tiles_k, p.run };
+    const dim3 grid((unsigned)((int64_t)p.splits * p.tiles_n * tiles_k));
+    if (p.s == 64) k8_dw<T, 64, NP><<<grid, 512, 0, st>>>(d, o);
+    else if (p.s == 128) k8_dw<T, 128, NP><<<grid, 512, 0, st>>>(d, o);
+    else k8_dw<T, 256, NP><<<grid, 512, 0, st>>>(d, o);
+    if (p.splits > 1) {
+        if (d.dw) k8_dw_join<<<dim3((unsigned)(d.n * ((d.k + 255) / 256))), 256, 0, st>>>(o.part, p.splits, d.n, d.k, d.dw, d.dw_type, d.lddw);
+        if (d.db) k8_dw_join<<<dim3((unsigned)((d.n + 255) / 256)), 256, 0, st>>>(o.part_b, p.splits, 1, d.n, d.db, d.dw_type, d.n);
+    }
+    return hipGetLastError();
 }
 
 }  // namespace
 
-#define K8_TYPE(type_, T_, ...) \
-    switch (type_) { case DN_T_F32: { typedef float T_; __VA_ARGS__; break; } case DN_T_F16: { typedef _Float16 T_; __VA_ARGS__; break; } \
-                     default: { typedef k8_bf16 T_; __VA_ARGS__; break; } }
+uint64_t k8_grad_workspace(const dn_i8_grad_desc &d) { return plan_grad(d).total; }
 
-uint64_t k8_grad_workspace(const dn_i8_grad_desc &) { return 0; }
-
-hipError_t k8_grad(const dn_i8_grad_desc &d, void *, hipStream_t st) {
-    const int64_t kb = (d.k + 255) / 256;
-    K8_TYPE(d.dy_type, T,
-            if (d.dx && d.m) k8_dx_k<T><<<dim3((unsigned)(d.m * kb)), 256, 0, st>>>(d);
-            if (d.dw || d.db) K8_TYPE(d.dw_type, W, k8_dw_k<T, W><<<dim3((unsigned)(d.n * kb)), 256, 0, st>>>(d)));
-    return hipGetLastError();
+template <class T> static hipError_t grad_of(const dn_i8_grad_desc &d, const Plan &p, char *base, hipStream_t st) {
+    hipError_t e = hipSuccess;
+    if (d.dx && d.m) e = dx_of<T, sizeof(T) / 2>(d, p, base, st);
+    if (e == hipSuccess && (d.dw || d.db)) e = p.np_w == 2 ? dw_of<T, 2>(d, p, base, st) : dw_of<T, 1>(d, p, base, st);
+    return e;
+}
+hipError_t k8_grad(const dn_i8_grad_desc &d, void *ws, hipStream_t st) {
+    const Plan p = plan_grad(d);
+    switch (d.dy_type) {
+        case DN_T_F32: return grad_of<float>(d, p, (char *)ws, st);
+        case DN_T_F16: return grad_of<_Float16>(d, p, (char *)ws, st);
+        default: return grad_of<k8_bf16>(d, p, (char *)ws, st);
+    }
 }

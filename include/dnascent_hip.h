@@ -282,6 +282,7 @@ int dn_debug_emission(dn_ctx *ctx, uint32_t n, const double *x, const double *mu
 enum { DN_T_F32 = 0, DN_T_F16 = 1, DN_T_BF16 = 2, DN_T_I8 = 3 };
 #define DN_I8_MAX_K 131071               /* 128 * 128 * K stays below 2^31 */
 #define DN_I8_MAX_M 2147483136ll
+#define DN_I8_MAX_PITCH 8388608ll        /* bytes between a matrix's rows */
 /* rows of x (x_type DN_T_F32 / F16 / BF16) -> q, s.  ldq >= k; the bytes of q behind k up to the next multiple of 16 (or ldq, if that is nearer) become 0. */
 int dn_i8_rows(dn_ctx *ctx, int64_t m, int64_t k, const void *x, int64_t ldx, int x_type, int8_t *q, int64_t ldq, float *s, void *hip_stream);
 /* q s -> x, rounded once to x_type */

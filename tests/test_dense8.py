@@ -35,7 +35,7 @@ def _ask(entry, d):
 @pytest.mark.parametrize("kw", [
     dict(), dict(m=0, x=None, y=None), dict(m=1, ldx=0), dict(ldx=0), dict(bias=P), dict(residual=P, ldr=7), dict(relu=1, mask=P, ldmask=1),
     dict(q=P, ldq=33, s=P), dict(x_type=3, sx=P), dict(x_type=1, y_type=2), dict(n=131071, ldy=131071), dict(k=131071, ldx=131071, ldw=131071),
-    dict(m=2147483135)])
+    dict(m=2147483135), dict(ldx=1 << 21)])
 def test_linear_takes(kw):
     assert _ask("dn_i8_linear", _linear(**kw))[0] == 0
 
@@ -45,7 +45,7 @@ def test_linear_takes(kw):
     dict(x_type=4), dict(x_type=-1), dict(y_type=3), dict(relu=2), dict(reserved=1),                                               # types and flags
     dict(x=None), dict(w=None), dict(sw=None), dict(y=None), dict(x=P + 2), dict(y=P + 1), dict(sw=P + 2), dict(bias=P + 1),       # missing, misaligned
     dict(x_type=1, x=P + 1), dict(ldx=32), dict(ldx=-1), dict(ldw=32), dict(ldy=6), dict(ldy=0), dict(residual=P, ldr=3),          # pitches
-    dict(m=1, ldy=6), dict(ldx=1 << 31),
+    dict(m=1, ldy=6), dict(ldx=1 << 31), dict(ldx=(1 << 21) + 1),
     dict(x_type=3), dict(sx=P), dict(mask=P, ldmask=1), dict(relu=1, mask=P, ldmask=0), dict(q=P, ldq=33), dict(s=P), dict(q=P, ldq=32, s=P),
     dict(x_type=3, sx=P, q=P, ldq=33, s=P)])
 def test_linear_refuses(kw):
