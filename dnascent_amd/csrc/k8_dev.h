@@ -11,6 +11,9 @@ template <class T, int N> struct __attribute__((packed, aligned(sizeof(T)))) K8V
 template <class T, int N> __device__ __forceinline__ K8Vec<T, N> k8_load(const T *p) { return *(const K8Vec<T, N> *)p; }
 template <class T, int N> __device__ __forceinline__ void k8_store(T *p, const K8Vec<T, N> &v) { *(K8Vec<T, N> *)p = v; }
 
+typedef unsigned __attribute__((ext_vector_type(2), aligned(1))) k8_u32x2;
+typedef unsigned __attribute__((ext_vector_type(4), aligned(1))) k8_u32x4;
+typedef unsigned __attribute__((aligned(1))) k8_u32;
 // N numbers of T as the dwords they lie in: 16-bit numbers stay two to a register
 template <class T, int N> struct K8Raw {
     unsigned w[N * sizeof(T) / 4];
@@ -30,6 +33,17 @@ template <class T, int N> struct K8Raw {
                 else w[e / 2] |= (unsigned)*(const uint16_t *)(p + e) << (16 * (e & 1));
             }
     }
+    __device__ __forceinline__ void load(k8_global p) {
+        if constexpr (sizeof w == 8) { const k8_u32x2 v = *(const __attribute__((address_space(1))) k8_u32x2 *)p; w[0] = v[0]; w[1] = v[1]; }
+        else
+#pragma unroll
+            for (unsigned i = 0; i < sizeof w / 16; i++) {
+                const k8_u32x4 v = *(const __attribute__((address_space(1))) k8_u32x4 *)(p + 16 * i);
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[4 * i + j] = v[j];
+            }
+    }
+    __device__ __forceinline__ void load(k8_global p, int have) { load((const T *)(const char *)p, have); }
     // the compiler knows nothing of what it computed from these registers before: it forms the values again instead of keeping them
     __device__ __forceinline__ void opaque() {
 #pragma unroll

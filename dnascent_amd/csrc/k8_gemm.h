@@ -42,6 +42,10 @@ __device__ __forceinline__ const char *k8_uniform(const char *p) {
     return (const char *)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)v));
 }
 
+// global memory behind a uniform address: one 32-bit offset per lane does, and the loads are global ones (a pointer made from integers alone is a generic one)
+typedef const __attribute__((address_space(1))) char *k8_global;
+__device__ __forceinline__ k8_global k8_base(const void *p) { return (k8_global)k8_uniform((const char *)p); }
+
 // which tile a workgroup takes.  Workgroups are dealt to the eight XCDs round-robin: XCD x takes a contiguous run of tiles, and inside the run tiles go
 // column block by column block over groups of eight row blocks, so that what an XCD works on at a time shares rows of a and of b in its own L2
 struct K8Tile { int tm, tn, z; };

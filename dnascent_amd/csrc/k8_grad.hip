@@ -16,6 +16,7 @@ __device__ __forceinline__ k8_f32x4 k8_mfma16(i32x4 a, i32x4 b, k8_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(k8_f16x8, a), __builtin_bit_cast(k8_f16x8, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ int k8_pack(float a, float b) { return __builtin_bit_cast(int, k8_f16x2{ (_Float16)a, (_Float16)b }); }
+__device__ __forceinline__ void k8_opaque(unsigned &v) { asm volatile("" : "+v"(v)); }
 // two numbers as two fp16 pieces each.  `hi` is hidden from the compiler: left to itself it forms the fp16 value that is subtracted with an instruction that rounds
 // the product behind v once, and stores the one that rounds twice.  Behind infinity and NaN there is nothing to add
 struct K8Split { int hi, lo; };
@@ -76,60 +77,88 @@ __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d) {
     }
     for (int i = threadIdx.x; i < NS * 32; i += 512) lsw[i] = i < n ? d.sw[i] : 0.0f;
     __syncthreads();
-    const int64_t tiles = (d.m + 16 * MT - 1) / (16 * MT), stride = (int64_t)gridDim.x * 8;
+    // a lane's places behind a row's end hold no number: `real` has a bit for each that does (byte s of the pair: step s)
+    unsigned real[2] = { 0u, 0u };
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+        const int have = min(max(n - (s * 32 + 8 * g), 0), 8);
+        real[s / 4] |= ((1u << have) - 1u) << (8 * (s % 4));
+    }
     K8Raw<T, 8> raw[MT][NS];
     unsigned bit[MT][NS];
-    auto fetch = [&](int64_t tile) __attribute__((always_inline)) {
+    const bool masked = d.mask != nullptr;
+    // WHOLE: seven more rows lie behind the tile, so that eight numbers can be read at once wherever a row ends (and a lane that has none there reads its row's first)
+    auto fetch = [&](int64_t tile, auto kind) __attribute__((always_inline)) {
+        constexpr bool WHOLE = decltype(kind)::value;
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-            const int64_t row = min((tile * MT + i) * 16 + c, d.m - 1);
-            const T *p = (const T *)d.dy + row * d.ldy;
+            const int64_t first = (tile * MT + i) * 16;
+            const unsigned r = WHOLE ? (unsigned)c : (unsigned)min((int64_t)c, max(d.m - 1 - first, (int64_t)0));
+            const int64_t at0 = WHOLE ? first : min(first, d.m - 1);
+            const k8_global p = k8_base((const char *)d.dy + at0 * d.ldy * (int64_t)sizeof(T));
+            const unsigned row = r * (unsigned)d.ldy * (unsigned)sizeof(T);
 #pragma unroll
             for (int s = 0; s < NS; s++) {
                 const int at = s * 32 + 8 * g;
-                if (at + 8 <= n) raw[i][s].load(p + at);
-                else raw[i][s].load(p + at, n - at);
-                bit[i][s] = d.mask && at < n ? d.mask[row * d.ldmask + (at >> 3)] : 255u;
+                if (WHOLE) raw[i][s].load(p + (row + (unsigned)((at < n ? at : 0) * (int)sizeof(T))));
+                else raw[i][s].load(p + (row + (unsigned)(at * (int)sizeof(T))), n - at);
+            }
+            if (masked) {
+                const k8_global pm = k8_base(d.mask + at0 * d.ldmask);
+#pragma unroll
+                for (int s = 0; s < NS; s++) {
+                    const int at = (s * 32 + 8 * g) >> 3;
+                    bit[i][s] = *(const __attribute__((address_space(1))) unsigned char *)(pm + (r * (unsigned)d.ldmask + (unsigned)(at * 8 < n ? at : 0)));
+                }
             }
         }
     };
-    int64_t tile = (int64_t)blockIdx.x * 8 + wave;
-    if (tile < tiles) fetch(tile);
-    for (; tile < tiles; tile += stride) {
+    auto work = [&](int64_t tile, auto &&next) __attribute__((always_inline)) {
         i32x4 a[MT][NP][NS];
         float down[MT];
 #pragma unroll
         for (int i = 0; i < MT; i++) {
-            // the row's largest dz sw, then the pieces under its power of two.  (dz sw is formed twice: the products are cheaper than the registers.)
-            auto value = [&](int s, int e, const K8Vec<float, 8> &sw) { return (bit[i][s] >> e & 1 ? raw[i][s].get(e) : 0.0f) * sw.v[e]; };
-            unsigned top = 0;
+            unsigned kept[NS];
 #pragma unroll
             for (int s = 0; s < NS; s++) {
-                const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + 8 * g);
-#pragma unroll
-                for (int e = 0; e < 8; e++) top = max(top, k8_mag(value(s, e, sw)));
+                kept[s] = real[s / 4] >> (8 * (s % 4));
+                if (masked) kept[s] &= bit[i][s];
             }
-            top = max(top, (unsigned)__shfl_xor((int)top, 16));
-            top = max(top, (unsigned)__shfl_xor((int)top, 32));
-            if (__any(top >= 0x7f800000u)) {               // not finite: the others' power of two is taken from the finite ones
-                top = 0;
+            // the row's largest dz sw, then the pieces under its power of two.  (dz sw is formed twice: the products are cheaper than the registers.)
+            auto value = [&](int s, int e, const K8Vec<float, 8> &sw) __attribute__((always_inline)) {
+                return __uint_as_float(__float_as_uint(raw[i][s].get(e)) & (unsigned)((int)(kept[s] << (31 - e)) >> 31)) * sw.v[e];
+            };
+            unsigned here = 8 * g;                         // hidden: the 64 factors are read again for every tile instead of being kept
+            k8_opaque(here);
+            float most = 0.0f;                             // (the larger of a number and NaN is the number)
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + here);
+#pragma unroll
+                for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(value(s, e, sw)));
+            }
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            if (__any(most > 0x1.fffffep127f)) {           // infinite: the power of two comes from the finite ones
+                most = 0.0f;
 #pragma unroll
                 for (int s = 0; s < NS; s++) {
-                    const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + 8 * g);
+                    const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + here);
+                    raw[i][s].opaque(); k8_opaque(kept[s]);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) { const unsigned v = k8_mag(value(s, e, sw)); top = max(top, v < 0x7f800000u ? v : 0u); }
+                    for (int e = 0; e < 8; e++) { const float v = fabsf(value(s, e, sw)); most = fmaxf(most, v <= 0x1.fffffep127f ? v : 0.0f); }
                 }
-                top = max(top, (unsigned)__shfl_xor((int)top, 16));
-                top = max(top, (unsigned)__shfl_xor((int)top, 32));
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
             }
-            const K8Pow pw = k8_pow(top);
+            const K8Pow pw = k8_pow(__float_as_uint(most));
             down[i] = pw.down;
+            __builtin_amdgcn_sched_barrier(0);
             // the second pass forms the products again from these registers: 64 of them kept as fp32 do not fit beside the rest
 #pragma unroll
-            for (int s = 0; s < NS; s++) raw[i][s].opaque();
-#pragma unroll
             for (int s = 0; s < NS; s++) {
-                const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + 8 * g);
+                raw[i][s].opaque(); k8_opaque(kept[s]); k8_opaque(here);
+                const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + here);
 #pragma unroll
                 for (int p = 0; p < 4; p++) {
                     const float v0 = value(s, 2 * p, sw) * pw.up, v1 = value(s, 2 * p + 1, sw) * pw.up;
@@ -138,9 +167,14 @@ __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d) {
                         a[i][0][s][p] = w.hi; a[i][NP - 1][s][p] = w.lo;
                     } else a[i][0][s][p] = k8_pack(v0, v1);
                 }
+                // made here and now: sunk behind the next tile's loads, they would keep this tile's numbers alive beside those
+#pragma unroll
+                for (int p = 0; p < NP; p++) asm volatile("" : "+v"(a[i][p][s]));
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (tile + stride < tiles) fetch(tile + stride);
+        next();
+        __builtin_amdgcn_sched_barrier(0);
         float rs[MT][4];
 #pragma unroll
         for (int i = 0; i < MT; i++)
@@ -161,6 +195,7 @@ __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d) {
 #pragma unroll
                         for (int p = 0; p < NP; p++) acc[i][t] = k8_mfma16(a[i][p][s], b, acc[i][t]);
                 }
+                __builtin_amdgcn_sched_barrier(0);         // a tile's fragments at a time: more of them in flight spill
             }
             const int64_t kk = k0 + blk * 64 + 4 * c;
 #pragma unroll
@@ -179,6 +214,14 @@ __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d) {
                         for (int t = 0; t < 4; t++) if (kk + t < d.k) p[t] = o.v[t];
                 }
         }
+    };
+    const int64_t tiles = (d.m + 16 * MT - 1) / (16 * MT), stride = (int64_t)gridDim.x * 8, whole = d.ldy ? max(d.m - 7, (int64_t)0) / (16 * MT) : 0;
+    int64_t tile = (int64_t)blockIdx.x * 8 + wave;
+    if (tile < whole) fetch(tile, std::true_type());
+    for (; tile < whole; tile += stride) work(tile, [&]() __attribute__((always_inline)) { if (tile + stride < whole) fetch(tile + stride, std::true_type()); });
+    for (; tile < tiles; tile += stride) {
+        fetch(tile, std::false_type());
+        work(tile, []() {});
     }
 }
 
@@ -362,8 +405,10 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
     K8Raw<T, 4> raw[8];
     unsigned rq[8], rbit[8];
     float rs[8];
-    // Row addresses are a uniform base and one 32-bit offset per lane and operand.  Rows behind the run repeat its last one and count as zeros (no mask bit, no scale)
-    const bool u_whole = ch + 4 <= ncols, q_whole = ch + 4 <= kcols, u_in = has_u && ch < ncols, q_in = has_q && with_q && ch < kcols;
+    // Two ways to fetch a tile.  WHOLE: all its rows are there and three more behind them, so that four channels can be read at once wherever a row ends (what lies
+    // behind it belongs to channels that are not stored); a lane's offset leads to its group's first row, the others follow by the base.  Otherwise row by row and
+    // channel by channel where a row ends; rows behind the run repeat its last one and count as zeros (no mask bit, no scale).
+    const bool u_in = has_u && ch < ncols, q_in = has_q && with_q && ch < kcols;
     const int esh = (int)((n0 + ch) & 7);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -371,42 +416,53 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
 #pragma unroll
         for (unsigned j = 0; j < sizeof(T); j++) raw[e].w[j] = 0u;
     }
-    auto fetch_rows = [&](int64_t base, auto full) __attribute__((always_inline)) {
-        constexpr bool FULL = decltype(full)::value;
-        const char *pu = k8_uniform((const char *)d.dy + (base * d.ldy + n0) * (int64_t)sizeof(T)), *pq = k8_uniform((const char *)d.q + base * d.ldq + k0);
-        const char *pm = k8_uniform((const char *)d.mask + base * d.ldmask + (n0 >> 3)), *ps = k8_uniform((const char *)(d.s + base));
+    typedef const __attribute__((address_space(1))) unsigned char *gu8;
+    typedef const __attribute__((address_space(1))) float *gf32;
+    auto fetch = [&](int64_t base, auto kind) __attribute__((always_inline)) {
+        constexpr bool WHOLE = decltype(kind)::value;
         const int left = (int)min(r1 - base, (int64_t)D::RT) - 1;
+        auto row = [&](int e) { return WHOLE ? (unsigned)(rg * 8) : (unsigned)min(rg * 8 + e, left); };
+        auto up = [&](int e) { return WHOLE ? (int64_t)e : (int64_t)0; };
+        if (u_in) {
+            const k8_global pu = k8_base((const char *)d.dy + (base * d.ldy + n0) * (int64_t)sizeof(T));
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            // FULL: lane offset to the group's first row, the other rows by the base; else every row by itself
-            const unsigned r = FULL ? (unsigned)(rg * 8) : (unsigned)min(rg * 8 + e, left);
-            const int64_t up = FULL ? e : 0;
-            if (u_in) {
-                if (with_q) rs[e] = *(const float *)(ps + up * 4 + r * 4u);
-                const T *p = (const T *)(pu + up * d.ldy * (int64_t)sizeof(T) + (r * (unsigned)d.ldy + (unsigned)ch) * (unsigned)sizeof(T));
-                if (u_whole) raw[e].load(p);
+            for (int e = 0; e < 8; e++) {
+                const k8_global p = pu + up(e) * d.ldy * (int64_t)sizeof(T) + (row(e) * (unsigned)d.ldy + (unsigned)ch) * (unsigned)sizeof(T);
+                if (WHOLE || ch + 4 <= ncols) raw[e].load(p);
                 else raw[e].load(p, ncols - ch);
-                if (d.mask) rbit[e] = (unsigned)*(const uint8_t *)(pm + up * d.ldmask + r * (unsigned)d.ldmask + (unsigned)(ch >> 3)) >> esh;
-                if (!FULL && rg * 8 + e > left) { rbit[e] = 0u; rs[e] = 0.0f; }
-                else if (!FULL && !d.mask) rbit[e] = 255u;
             }
-            if (q_in) {
-                const char *p = pq + up * d.ldq + r * (unsigned)d.ldq + (unsigned)ch;
-                if (q_whole) __builtin_memcpy(&rq[e], p, 4);
+            if (d.mask) {
+                const k8_global pm = k8_base(d.mask + base * d.ldmask + (n0 >> 3));
+#pragma unroll
+                for (int e = 0; e < 8; e++) rbit[e] = (unsigned)*(gu8)(pm + up(e) * d.ldmask + (row(e) * (unsigned)d.ldmask + (unsigned)(ch >> 3)));
+            }
+            if (with_q) {
+                const k8_global ps = k8_base(d.s + base);
+#pragma unroll
+                for (int e = 0; e < 8; e++) rs[e] = *(gf32)(ps + up(e) * 4 + row(e) * 4u);
+            }
+        }
+        if (q_in) {
+            const k8_global pq = k8_base(d.q + base * d.ldq + k0);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const k8_global p = pq + up(e) * d.ldq + (row(e) * (unsigned)d.ldq + (unsigned)ch);
+                if (WHOLE || ch + 4 <= kcols) rq[e] = *(const __attribute__((address_space(1))) k8_u32 *)p;
                 else {
                     rq[e] = 0u;
 #pragma unroll
-                    for (int j = 0; j < 3; j++) if (ch + j < kcols) rq[e] |= (unsigned)*(const uint8_t *)(p + j) << (8 * j);
+                    for (int j = 0; j < 3; j++) if (ch + j < kcols) rq[e] |= (unsigned)((gu8)p)[j] << (8 * j);
                 }
             }
         }
-    };
-    auto fetch = [&](int64_t base) __attribute__((always_inline)) {
-        if (base + D::RT <= r1) fetch_rows(base, std::true_type());
-        else fetch_rows(base, std::false_type());
+        if (!WHOLE)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (rg * 8 + e > left) { rbit[e] = 0u; rs[e] = 0.0f; }
+                else if (!d.mask) rbit[e] = ch < ncols ? 255u : 0u;
     };
     float pw[4] = { 0x1p126f, 0x1p126f, 0x1p126f, 0x1p126f }, sum[4] = { 0, 0, 0, 0 };
-    auto dz = [&](int e, int j) { return rbit[e] >> j & 1 ? raw[e].get(j) : 0.0f; };
+    auto dz = [&](int e, int j) { return rbit[e] >> (esh + j) & 1 ? raw[e].get(j) : 0.0f; };
     // the turned fp16 values of this thread's task (and, the first time, the sums of dz); true if one does not fit
     auto make = [&](char *l, auto first) __attribute__((always_inline)) {
         float most = 0.0f;
@@ -461,9 +517,8 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
                 for (int j = 0; j < TK; j++) acc[i][j] = k8_mfma16(a[i], b[j], acc[i][j]);
         }
     };
-    if (r0 < r1) fetch(r0);                                // (a call without rows has one empty run: its sums are zeros)
     int stage = 0;
-    for (int64_t base = r0; base < r1; base += D::RT, stage ^= 1) {
+    auto tile = [&](auto &&next) __attribute__((always_inline)) {
         char *l = lds[stage];
         const bool over = make(l, std::true_type());
         if (with_q) {
@@ -509,8 +564,18 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
                 __syncthreads();
             }
         }
-        if (base + D::RT < r1) fetch(base + D::RT);
+        next();
         if (with_q) multiply(l);
+        stage ^= 1;
+    };
+    // (a call without rows has one empty run: its sums are zeros)
+    int64_t base = r0;
+    const int64_t whole = min(r1, d.ldy && d.ldq ? d.m - 3 : (int64_t)0) - D::RT;         // the last tile that can be fetched whole starts here or before
+    if (base <= whole) fetch(base, std::true_type());
+    for (; base <= whole; base += D::RT) tile([&]() __attribute__((always_inline)) { if (base + D::RT <= whole) fetch(base + D::RT, std::true_type()); });
+    for (; base < r1; base += D::RT) {
+        fetch(base, std::false_type());
+        tile([]() {});
     }
     // ---- the sums leave: sets of wavefronts joined in LDS first, in the order of the sets
     __syncthreads();
