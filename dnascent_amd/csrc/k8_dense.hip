@@ -11,12 +11,12 @@ template <class T, int LPR, int V, int R>
 __global__ __launch_bounds__(256) void k8_rows_k(int64_t m, int k, const T *__restrict__ x, int64_t ldx, int8_t *__restrict__ q, int64_t ldq, float *__restrict__ s) {
     constexpr int E = 16 / sizeof(T);
     const int lid = threadIdx.x % LPR;
-    const int64_t row0 = ((int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR) * R;
+    const int64_t row0 = (int64_t)blockIdx.x * (256 / LPR) * R + threadIdx.x / LPR;      // row i of a lane group: adjacent groups hold adjacent rows
     K8Vec<T, E> raw[R][V];
     unsigned top[R];
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        const T *xr = x + min(row0 + i, m - 1) * ldx;
+        const T *xr = x + min(row0 + i * (256 / LPR), m - 1) * ldx;
 #pragma unroll
         for (int v = 0; v < V; v++) {
             const int c = (v * LPR + lid) * E;
@@ -45,9 +45,10 @@ __global__ __launch_bounds__(256) void k8_rows_k(int64_t m, int k, const T *__re
     const int pad = (int)min((int64_t)((k + 15) & ~15), ldq);
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        if (row0 + i >= m) break;
+        const int64_t row = row0 + i * (256 / LPR);
+        if (row >= m) break;
         const K8Scale sc = k8_scale(top[i]);
-        int8_t *qr = q + (row0 + i) * ldq;
+        int8_t *qr = q + row * ldq;
 #pragma unroll
         for (int v = 0; v < V; v++) {
             const int c = (v * LPR + lid) * E;
@@ -60,7 +61,7 @@ __global__ __launch_bounds__(256) void k8_rows_k(int64_t m, int k, const T *__re
 #pragma unroll
                 for (int e = 0; e < E; e++) if (c + e < pad) qr[c + e] = (int8_t)(w.v[e / 4] >> (8 * (e % 4)));
         }
-        if (lid == 0) s[row0 + i] = sc.s;
+        if (lid == 0) s[row] = sc.s;
     }
 }
 // rows that do not fit a workgroup's registers: read twice (the second time mostly from cache)
@@ -123,13 +124,13 @@ template <class T, int LPR, int R>
 __global__ __launch_bounds__(256) void k8_restore_k(int64_t m, int k, const int8_t *__restrict__ q, int64_t ldq, const float *__restrict__ s, T *__restrict__ x, int64_t ldx) {
     constexpr int E = 16 / sizeof(T);
     const int lid = threadIdx.x % LPR;
-    const int64_t row0 = ((int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR) * R;
+    const int64_t row0 = (int64_t)blockIdx.x * (256 / LPR) * R + threadIdx.x / LPR;
     for (int c = lid * E; c < k; c += LPR * E) {
         K8Vec<int8_t, E> raw[R];
         float sc[R];
 #pragma unroll
         for (int i = 0; i < R; i++) {
-            const int64_t row = min(row0 + i, m - 1);
+            const int64_t row = min(row0 + i * (256 / LPR), m - 1);
             sc[i] = s[row];
             if (c + E <= k) raw[i] = k8_load<int8_t, E>(q + row * ldq + c);
             else
@@ -138,12 +139,13 @@ __global__ __launch_bounds__(256) void k8_restore_k(int64_t m, int k, const int8
         }
 #pragma unroll
         for (int i = 0; i < R; i++) {
-            if (row0 + i >= m) break;
-            T *xr = x + (row0 + i) * ldx + c;
+            const int64_t row = row0 + i * (256 / LPR);
+            if (row >= m) break;
+            T *xr = x + row * ldx + c;
             K8Vec<T, E> o;
 #pragma unroll
             for (int e = 0; e < E; e++) o.v[e] = (T)((float)raw[i].v[e] * sc[i]);
-            if (c + E <= k) k8_store<T, E>(xr, o);
+            if (c + E <= k) k8_stream<T, E>(xr, o);
             else
 #pragma unroll
                 for (int e = 0; e < E; e++) if (c + e < k) xr[e] = o.v[e];
@@ -157,7 +159,8 @@ hipError_t restore_of(int64_t m, int k, const int8_t *q, int64_t ldq, const floa
     if (pieces <= 8) REST(8, 4);
     else if (pieces <= 16) REST(16, 4);
     else if (pieces <= 32) REST(32, 4);
-    else if (m >= 8 * K8_CUS) REST(64, 4);
+    else if (pieces <= 64 && m >= 8 * K8_CUS) REST(64, 4);
+    else if (m >= 8 * K8_CUS) REST(64, 1);
     else REST(256, 1);
 #undef REST
     return hipGetLastError();
@@ -189,7 +192,7 @@ __device__ __forceinline__ void k8_put(const Out &o, int64_t mm, int64_t nn, flo
 #pragma unroll
     for (int j = 0; j < TN; j++) y.v[j] = (T)(o.relu ? k8_relu(v[j]) : v[j]);
     T *p = (T *)o.y + mm * o.ldy + nn;
-    if (nn + TN <= o.n) k8_store<T, TN>(p, y);
+    if (nn + TN <= o.n) k8_stream<T, TN>(p, y);
     else
 #pragma unroll
         for (int j = 0; j < TN; j++) if (nn + j < o.n) p[j] = y.v[j];
@@ -293,40 +296,69 @@ __global__ __launch_bounds__(512) void k8_few(const X *__restrict__ x, int64_t l
     extern __shared__ __align__(16) char dyn[];            // X != int8_t: the rows' codes at a pitch of kp + 16 bytes
     __shared__ int sums[8][MT * 256];
     __shared__ float scales[MT * 16];
+    __shared__ unsigned tops[8];
     constexpr bool GIVEN = sizeof(X) == 1;
     const int lane = threadIdx.x & 63, wave = k8_uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4, m = (int)o.m;
     const int kp = (k + 63) & ~63, pitch = kp + 16, mine = min(c, m - 1);      // operand rows behind the last one repeat it
     const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const int steps = kp >> 6, whole = k >> 6;             // whole: steps that no lane has to cut
+    const int8_t *wr = w + min(n0 + c, o.n - 1) * ldw;
+    // the first eight steps of the weight are asked for before anything else
+    i32x4 b[8];
+    const bool eight = wave + 56 < whole;
+    if (eight)
+#pragma unroll
+        for (int u = 0; u < 8; u++) b[u] = __builtin_bit_cast(i32x4, k8_load<int8_t, 16>(wr + (wave + 8 * u) * 64 + g * 16));
     if constexpr (GIVEN) {
         if (threadIdx.x < MT * 16) scales[threadIdx.x] = o.sx[min((int)threadIdx.x, m - 1)];
     } else {
-        for (int r = wave; r < m; r += 8) {
-            const X *xr = x + r * ldx;
+        // 8, 4, 2 or 1 wavefronts a row; M K <= 16384, so that a lane holds its share of a row in eight pieces of eight numbers at most
+        const int per = m == 1 ? 8 : m == 2 ? 4 : m <= 4 ? 2 : 1, part = wave % per;
+        for (int r = wave / per; r < (m + 8 / per - 1) / (8 / per) * (8 / per); r += 8 / per) {      // (as many rounds for every wavefront)
+            const X *xr = x + min(r, m - 1) * ldx;
+            K8Raw<X, 8> raw[8];
             unsigned top = 0;
-            for (int i = lane * 4; i < kp; i += 256)
 #pragma unroll
-                for (int e = 0; e < 4; e++) top = max(top, i + e < k ? k8_mag((float)xr[i + e]) : 0u);
-            for (int b = 32; b; b >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, b));
+            for (int v = 0; v < 8; v++) {
+                const int at = ((v * per + part) * 64 + lane) * 8;
+                if (at + 8 <= k) raw[v].load(xr + at);
+                else if (v * per * 512 < k) raw[v].load(xr + at, k - at);
+                else raw[v] = {};
+            }
+#pragma unroll
+            for (int v = 0; v < 8; v++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = max(top, k8_mag(raw[v].get(e)));
+            for (int d = 32; d; d >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, d));
+            if (per > 1) {
+                if (lane == 0) tops[wave] = top;
+                __syncthreads();
+                for (int z = 0; z < per; z++) top = max(top, tops[wave / per * per + z]);
+            }
+            if (r >= m) break;                             // (only where a wavefront has a row to itself: no barrier follows)
             const K8Scale sc = k8_scale(top);
             const int pad = (int)min((int64_t)((k + 15) & ~15), ldq);
-            for (int i = lane * 4; i < kp; i += 256) {
-                float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = i + e < k ? (float)xr[i + e] : 0.0f;
-                const unsigned q = k8_codes(v[0], v[1], v[2], v[3], sc.r);
-                *(unsigned *)(dyn + r * pitch + i) = q;
-                if (qout && blockIdx.x == 0)
+            for (int v = 0; v < 8; v++) {
+                const int at = ((v * per + part) * 64 + lane) * 8;
+                if (at >= kp) break;
+                const unsigned q0 = k8_codes(raw[v].get(0), raw[v].get(1), raw[v].get(2), raw[v].get(3), sc.r);
+                const unsigned q1 = k8_codes(raw[v].get(4), raw[v].get(5), raw[v].get(6), raw[v].get(7), sc.r);
+                *(uint2 *)(dyn + r * pitch + at) = make_uint2(q0, q1);
+                if (qout && blockIdx.x == 0) {
+                    if (at + 8 <= pad) { const uint2 q = make_uint2(q0, q1); __builtin_memcpy(qout + r * ldq + at, &q, 8); }
+                    else
 #pragma unroll
-                    for (int e = 0; e < 4; e++) if (i + e < pad) qout[r * ldq + i + e] = (int8_t)(q >> (8 * e));
+                        for (int e = 0; e < 8; e++) if (at + e < pad) qout[r * ldq + at + e] = (int8_t)((e < 4 ? q0 : q1) >> (8 * (e & 3)));
+                }
             }
-            if (lane == 0) { scales[r] = sc.s; if (sout && blockIdx.x == 0) sout[r] = sc.s; }
+            if (lane == 0 && part == 0) { scales[r] = sc.s; if (sout && blockIdx.x == 0) sout[r] = sc.s; }
         }
         __syncthreads();
     }
     i32x4 acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; t++) acc[t] = i32x4{ 0, 0, 0, 0 };
-    const int8_t *wr = w + min(n0 + c, o.n - 1) * ldw;
     const int8_t *xr[MT];
 #pragma unroll
     for (int t = 0; t < MT; t++) xr[t] = GIVEN ? (const int8_t *)x + min(t * 16 + c, m - 1) * ldx : nullptr;
@@ -337,10 +369,9 @@ __global__ __launch_bounds__(512) void k8_few(const X *__restrict__ x, int64_t l
         for (int e = 0; e < 16; e++) v.v[e] = at + e < k ? row[at + e] : (int8_t)0;
         return __builtin_bit_cast(i32x4, v);
     };
-    const int steps = kp >> 6, whole = k >> 6;             // whole: steps that no lane has to cut
     int s = wave;
     for (; s + 56 < whole; s += 64) {
-        i32x4 b[8];
+        if (s != wave)
 #pragma unroll
         for (int u = 0; u < 8; u++) b[u] = __builtin_bit_cast(i32x4, k8_load<int8_t, 16>(wr + (s + 8 * u) * 64 + g * 16));
 #pragma unroll
@@ -354,12 +385,12 @@ __global__ __launch_bounds__(512) void k8_few(const X *__restrict__ x, int64_t l
     }
     for (; s < steps; s += 8) {
         const int at = s * 64 + g * 16;
-        const i32x4 b = piece(wr, at);
+        const i32x4 bp = piece(wr, at);
 #pragma unroll
         for (int t = 0; t < MT; t++) {
             i32x4 a;
             if constexpr (GIVEN) a = piece(xr[t], at); else a = *(const i32x4 *)(dyn + mine * pitch + at);
-            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, bp, acc[t], 0, 0, 0);
         }
     }
 #pragma unroll

@@ -14,6 +14,12 @@ template <class T, int N> __device__ __forceinline__ void k8_store(T *p, const K
 typedef unsigned __attribute__((ext_vector_type(2), aligned(1))) k8_u32x2;
 typedef unsigned __attribute__((ext_vector_type(4), aligned(1))) k8_u32x4;
 typedef unsigned __attribute__((aligned(1))) k8_u32;
+// results that are not read again soon: past the caches
+template <class T, int N> __device__ __forceinline__ void k8_stream(T *p, const K8Vec<T, N> &v) {
+    if constexpr (sizeof v == 16) { k8_u32x4 w; __builtin_memcpy(&w, &v, 16); __builtin_nontemporal_store(w, (k8_u32x4 *)p); }
+    else if constexpr (sizeof v == 8) { k8_u32x2 w; __builtin_memcpy(&w, &v, 8); __builtin_nontemporal_store(w, (k8_u32x2 *)p); }
+    else k8_store<T, N>(p, v);
+}
 // N numbers of T as the dwords they lie in: 16-bit numbers stay two to a register
 template <class T, int N> struct K8Raw {
     unsigned w[N * sizeof(T) / 4];

@@ -633,32 +633,46 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
         }
     }
 }
-// the runs joined: 64 lanes x four adjacent results, four wavefronts a quarter of the runs each
-__global__ __launch_bounds__(256) void k8_dw_join(const float *__restrict__ part, int splits, int64_t rows, int64_t k, void *__restrict__ out, int type, int64_t ld) {
-    __shared__ float js[4][64][4];
-    const int64_t kb = (k + 255) / 256, r = blockIdx.x / kb, kk = (blockIdx.x % kb) * 256 + (threadIdx.x & 63) * 4;
+// the runs joined, dw's and db's in one launch.  A workgroup takes 256 adjacent results: 64 lanes x four, 16 wavefronts a sixteenth of the runs each, so that a
+// run's loads are all in flight at once
+__global__ __launch_bounds__(1024) void k8_dw_join(const float *__restrict__ part, const float *__restrict__ part_b, int splits, int64_t n, int64_t k, void *__restrict__ dw,
+                                                   int64_t lddw, void *__restrict__ db, int type, unsigned dw_blocks) {
+    __shared__ float js[16][256];
+    const bool is_b = blockIdx.x >= dw_blocks;
+    const int64_t count = is_b ? n : n * k, at = (int64_t)(is_b ? blockIdx.x - dw_blocks : blockIdx.x) * 256;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t mine = at + lane * 4, left = count - mine;
     float v[4] = { 0, 0, 0, 0 };
-    if (kk < k)
-#pragma unroll 4
-        for (int z = wave; z < splits; z += 4) {
-            const float *p = part + ((int64_t)z * rows + r) * k + kk;
-            if (kk + 4 <= k) {
-                const K8Vec<float, 4> t = k8_load<float, 4>(p);
+    if (left > 0) {
+        const float *p = (is_b ? part_b : part) + mine;
+        for (int z0 = wave; z0 < splits; z0 += 256) {      // sixteen runs a wavefront, all of them asked for before the first is added
+            K8Vec<float, 4> t[16];
 #pragma unroll
-                for (int j = 0; j < 4; j++) v[j] += t.v[j];
-            } else
+            for (int u = 0; u < 16; u++) {
+                const float *q = p + (int64_t)min(z0 + 16 * u, splits - 1) * count;
+                if (left >= 4) t[u] = k8_load<float, 4>(q);
+                else
 #pragma unroll
-                for (int j = 0; j < 4; j++) if (kk + j < k) v[j] += p[j];
+                    for (int j = 0; j < 4; j++) t[u].v[j] = j < left ? q[j] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 16; u++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[j] += z0 + 16 * u < splits ? t[u].v[j] : 0.0f;
         }
-#pragma unroll
-    for (int j = 0; j < 4; j++) js[wave][lane][j] = v[j];
-    __syncthreads();
-    if (wave == 0 && kk < k) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = js[0][lane][j] + js[1][lane][j] + js[2][lane][j] + js[3][lane][j];
-        k8_put4(out, type, r * ld + kk, v, k - kk);
     }
+    *(k8_f32x4 *)(&js[wave][lane * 4]) = k8_f32x4{ v[0], v[1], v[2], v[3] };
+    __syncthreads();
+    const int64_t o = at + threadIdx.x;
+    if (threadIdx.x >= 256 || o >= count) return;
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; w++) s += js[w][threadIdx.x];
+    const int64_t to = is_b ? o : o / k * lddw + o % k;
+    void *out = is_b ? db : dw;
+    if (type == DN_T_F32) ((float *)out)[to] = s;
+    else if (type == DN_T_F16) ((_Float16 *)out)[to] = (_Float16)s;
+    else ((k8_bf16 *)out)[to] = (k8_bf16)s;
 }
 
 // ---- which way a call takes.  Nothing here looks at which results are asked for: a result's bits do not depend on its company -----------------------------------------
@@ -742,8 +756,8 @@ template <class T, int NP> hipError_t dw_of(const dn_i8_grad_desc &d, const Plan
     else if (p.s == 128) k8_dw<T, 128, NP><<<grid, 512, 0, st>>>(d, o);
     else k8_dw<T, 256, NP><<<grid, 512, 0, st>>>(d, o);
     if (p.splits > 1) {
-        if (d.dw) k8_dw_join<<<dim3((unsigned)(d.n * ((d.k + 255) / 256))), 256, 0, st>>>(o.part, p.splits, d.n, d.k, d.dw, d.dw_type, d.lddw);
-        if (d.db) k8_dw_join<<<dim3((unsigned)((d.n + 255) / 256)), 256, 0, st>>>(o.part_b, p.splits, 1, d.n, d.db, d.dw_type, d.n);
+        const unsigned dw_blocks = d.dw ? (unsigned)((d.n * d.k + 255) / 256) : 0, db_blocks = d.db ? (unsigned)((d.n + 255) / 256) : 0;
+        k8_dw_join<<<dim3(dw_blocks + db_blocks), 1024, 0, st>>>(o.part, o.part_b, p.splits, d.n, d.k, d.dw, d.lddw, d.db, d.dw_type, dw_blocks);
     }
     return hipGetLastError();
 }

@@ -4,6 +4,7 @@ There is no fallback: if the library is missing, or no gfx950 device is usable, 
 """
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -75,19 +76,22 @@ def cnn_ops_from_description(desc):
     return ops
 
 
-class I8Linear(C.Structure):
-    """dn_i8_linear_desc"""
-    _fields_ = [("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64), ("sx", C.c_void_p), ("w", C.c_void_p),
-                ("ldw", C.c_int64), ("sw", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("ldr", C.c_int64), ("y", C.c_void_p),
-                ("ldy", C.c_int64), ("mask", C.c_void_p), ("ldmask", C.c_int64), ("q", C.c_void_p), ("ldq", C.c_int64), ("s", C.c_void_p),
-                ("x_type", C.c_int32), ("y_type", C.c_int32), ("relu", C.c_int32), ("reserved", C.c_int32)]
+# dn_i8_linear_desc / dn_i8_grad_desc: their fields in the header's order, packed with struct (a call's description costs a fraction of a ctypes structure)
+I8_LINEAR_FIELDS = (("m", "q"), ("n", "q"), ("k", "q"), ("x", "P"), ("ldx", "q"), ("sx", "P"), ("w", "P"), ("ldw", "q"), ("sw", "P"), ("bias", "P"),
+                    ("residual", "P"), ("ldr", "q"), ("y", "P"), ("ldy", "q"), ("mask", "P"), ("ldmask", "q"), ("q", "P"), ("ldq", "q"), ("s", "P"),
+                    ("x_type", "i"), ("y_type", "i"), ("relu", "i"), ("reserved", "i"))
+I8_GRAD_FIELDS = (("m", "q"), ("n", "q"), ("k", "q"), ("dy", "P"), ("ldy", "q"), ("mask", "P"), ("ldmask", "q"), ("q", "P"), ("ldq", "q"), ("s", "P"),
+                  ("w", "P"), ("ldw", "q"), ("sw", "P"), ("dx", "P"), ("ldx", "q"), ("dw", "P"), ("lddw", "q"), ("db", "P"), ("dy_type", "i"), ("dw_type", "i"))
+I8_LINEAR = struct.Struct("@" + "".join(f for _, f in I8_LINEAR_FIELDS))
+I8_GRAD = struct.Struct("@" + "".join(f for _, f in I8_GRAD_FIELDS))
 
 
-class I8Grad(C.Structure):
-    """dn_i8_grad_desc"""
-    _fields_ = [("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("dy", C.c_void_p), ("ldy", C.c_int64), ("mask", C.c_void_p), ("ldmask", C.c_int64),
-                ("q", C.c_void_p), ("ldq", C.c_int64), ("s", C.c_void_p), ("w", C.c_void_p), ("ldw", C.c_int64), ("sw", C.c_void_p), ("dx", C.c_void_p),
-                ("ldx", C.c_int64), ("dw", C.c_void_p), ("lddw", C.c_int64), ("db", C.c_void_p), ("dy_type", C.c_int32), ("dw_type", C.c_int32)]
+def i8_desc(fields, **values):
+    """the packed description of a dn_i8_linear (fields = I8_LINEAR_FIELDS) or dn_i8_linear_grad (I8_GRAD_FIELDS) call; what is not given is 0 / NULL"""
+    unknown = set(values) - {n for n, _ in fields}
+    if unknown:
+        raise TypeError("no such field: %s" % ", ".join(sorted(unknown)))
+    return struct.pack("@" + "".join(f for _, f in fields), *[values.get(n) or 0 for n, _ in fields])
 
 
 SUMMARY_DTYPE = np.dtype([
@@ -167,14 +171,26 @@ def lib():
         L.dn_i8_rows.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]
         L.dn_i8_restore.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_void_p]
         for n in ("dn_i8_linear", "dn_i8_linear_grad"):
-            getattr(L, n).argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]
-            getattr(L, n + "_workspace").argtypes = [C.c_void_p, C.c_void_p, C.POINTER(C.c_uint64)]
+            getattr(L, n).argtypes = [C.c_void_p, C.c_char_p, C.c_void_p, C.c_uint64, C.c_void_p]
+            getattr(L, n + "_workspace").argtypes = [C.c_void_p, C.c_char_p, C.POINTER(C.c_uint64)]
         _lib = L
     return _lib
 
 
 class DnError(RuntimeError):
     pass
+
+
+_dense8_module = None
+
+
+def _dense8():
+    """dnascent_amd.dense8, imported with its torch when an 8-bit layer is first used"""
+    global _dense8_module
+    if _dense8_module is None:
+        from . import dense8
+        _dense8_module = dense8
+    return _dense8_module
 
 
 class Context:
@@ -395,26 +411,22 @@ class Context:
         """dn_i8_rows: x [..., K] (fp32, fp16 or bf16) as rows of 8-bit integers and one fp32 scale each -> (q [..., K] int8, s [...]).  A row of q
         starts at a multiple of 16 bytes (its pitch is K rounded up), which is how i8_linear and i8_linear_grad read rows fastest; a weight [N, K]
         becomes (wq, ws) the same way, once."""
-        from . import dense8
-        return dense8.rows(self, x)
+        return _dense8().rows(self, x)
 
     def i8_restore(self, q, s, dtype):
         """dn_i8_restore: the numbers that i8_rows' result stands for, q * s, rounded once to dtype."""
-        from . import dense8
-        return dense8.restore(self, q, s, dtype)
+        return _dense8().restore(self, q, s, dtype)
 
     def i8_linear(self, x, wq, ws, sx=None, bias=None, residual=None, relu=False, out_dtype=None, save=False):
         """dn_i8_linear: y [..., N] = act(x W^T + bias + residual) with x [..., K] in 8 bits: numbers (then their rows are made on the way), or int8 rows
         with their scales sx.  wq [N, K] int8, ws [N] fp32, bias [N] fp32, residual [..., N] of y's type.  out_dtype: x's type, or bf16 for int8 rows.
         save=True: (y, dense8.Saved) -- what i8_linear_grad needs: the rows, their scales and, with relu, one bit per output."""
-        from . import dense8
-        return dense8.linear(self, x, wq, ws, sx, bias, residual, relu, out_dtype, save)
+        return _dense8().linear(self, x, wq, ws, sx, bias, residual, relu, out_dtype, save)
 
     def i8_linear_grad(self, dy, q, s, wq, ws, mask=None, need_dx=True, need_dw=True, need_db=True, w_dtype=None):
         """dn_i8_linear_grad: (dx [..., K] of dy's type, dw [N, K], db [N], both of w_dtype: dy's type if not given) for dy [..., N] from the 8-bit rows
         of the layer's input; None for what is not needed.  mask: dense8.Saved.mask of a layer with a ReLU."""
-        from . import dense8
-        return dense8.linear_grad(self, dy, q, s, wq, ws, mask, need_dx, need_dw, need_db, w_dtype)
+        return _dense8().linear_grad(self, dy, q, s, wq, ws, mask, need_dx, need_dw, need_db, w_dtype)
 
     # ---- measurement ------------------------------------------------------------------------
     def profile(self, on=True):

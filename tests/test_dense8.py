@@ -2,6 +2,7 @@
 side's through tensors that never reach a device.  Nothing is launched."""
 import ctypes as C
 import os
+import struct
 import subprocess
 from types import SimpleNamespace
 
@@ -18,18 +19,18 @@ def _linear(**kw):
     d = dict(m=5, n=7, k=33, x=P, ldx=33, sx=None, w=P, ldw=48, sw=P, bias=None, residual=None, ldr=0, y=P, ldy=7, mask=None, ldmask=0, q=None, ldq=0,
              s=None, x_type=0, y_type=0, relu=0, reserved=0)
     d.update(kw)
-    return hip.I8Linear(**d)
+    return hip.i8_desc(hip.I8_LINEAR_FIELDS, **d)
 
 
 def _grad(**kw):
     d = dict(m=5, n=7, k=33, dy=P, ldy=7, mask=None, ldmask=0, q=P, ldq=48, s=P, w=P, ldw=48, sw=P, dx=P, ldx=33, dw=P, lddw=33, db=P, dy_type=0, dw_type=0)
     d.update(kw)
-    return hip.I8Grad(**d)
+    return hip.i8_desc(hip.I8_GRAD_FIELDS, **d)
 
 
 def _ask(entry, d):
     need = C.c_uint64(0)
-    return getattr(hip.lib(), entry + "_workspace")(None, C.byref(d), C.byref(need)), need.value
+    return getattr(hip.lib(), entry + "_workspace")(None, d, C.byref(need)), need.value
 
 
 @pytest.mark.parametrize("kw", [
@@ -70,24 +71,25 @@ def test_grad_refuses(kw):
 def test_null_arguments():
     L = hip.lib()
     n = C.c_uint64(0)
-    assert L.dn_i8_linear_workspace(None, None, C.byref(n)) == -3 and L.dn_i8_linear_workspace(None, C.byref(_linear()), None) == -3
-    assert L.dn_i8_linear(None, C.byref(_linear()), None, 0, None) == -3 and L.dn_i8_linear_grad(None, C.byref(_grad()), None, 0, None) == -3
+    assert L.dn_i8_linear_workspace(None, None, C.byref(n)) == -3 and L.dn_i8_linear_workspace(None, _linear(), None) == -3
+    assert L.dn_i8_linear(None, _linear(), None, 0, None) == -3 and L.dn_i8_linear_grad(None, _grad(), None, 0, None) == -3
     assert L.dn_i8_rows(None, 1, 1, P, 1, 0, P, 16, P, None) == -3 and L.dn_i8_restore(None, 1, 1, P, 16, P, P, 1, 0, None) == -3
 
 
 def test_description_layouts_match_the_header(tmp_path):
     src = tmp_path / "layout.c"
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "dnascent_hip.h"', 'int main(void) {']
-    for name, t in (("dn_i8_linear_desc", hip.I8Linear), ("dn_i8_grad_desc", hip.I8Grad)):
+    want = []
+    for name, fields in (("dn_i8_linear_desc", hip.I8_LINEAR_FIELDS), ("dn_i8_grad_desc", hip.I8_GRAD_FIELDS)):
         lines.append('printf("%%zu\\n", sizeof(%s));' % name)
-        lines += ['printf("%%zu\\n", offsetof(%s, %s));' % (name, f[0]) for f in t._fields_]
+        lines += ['printf("%%zu\\n", offsetof(%s, %s));' % (name, f) for f, _ in fields]
+        code = "".join(f for _, f in fields)
+        want += [struct.calcsize("@" + code)] + [struct.calcsize("@" + code[:i + 1]) - struct.calcsize("@" + code[i]) for i in range(len(code))]
     src.write_text("\n".join(lines + ['return 0; }']))
     exe = tmp_path / "layout"
     subprocess.check_call(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)])
-    want = []
-    for t in (hip.I8Linear, hip.I8Grad):
-        want += [C.sizeof(t)] + [getattr(t, f[0]).offset for f in t._fields_]
     assert [int(v) for v in subprocess.check_output([str(exe)]).decode().split()] == want
+    assert (hip.I8_LINEAR.size, hip.I8_GRAD.size) == (want[0], want[len(hip.I8_LINEAR_FIELDS) + 1])
 
 
 def test_how_rows_lie():
@@ -104,8 +106,10 @@ def test_how_rows_lie():
                 torch.zeros(40).as_strided((5, 10), (4, 1))):
         with pytest.raises(ValueError):
             dense8._rows("t", bad)
-    q = dense8._empty_rows((3, 2, 33), "cpu")
-    assert q.shape == (3, 2, 33) and dense8._rows("q", q) == (6, 33, 48) and dense8._pitch(q) == 48
+    q, pitch = dense8._empty_rows((3, 2, 33), "cpu")
+    assert q.shape == (3, 2, 33) and dense8._rows("q", q) == (6, 33, 48) and pitch == 48
+    q, pitch = dense8._empty_rows((5, 32), "cpu")
+    assert q.shape == (5, 32) and dense8._rows("q", q) == (5, 32, 32) and pitch == 32
 
 
 def test_tensors_of_another_device_are_refused():

@@ -399,13 +399,13 @@ def test_outputs_end_where_they_end(ctx):
         q = torch.full((m + 2, k + 40), 77, dtype=torch.int8, device="cuda")
         s = torch.full((m + 2,), 7.0, device="cuda")
         mask = torch.full((m + 2, (n + 7) // 8 + 3), 0xA5, dtype=torch.uint8, device="cuda")
-        d = hip.I8Linear(m=m, n=n, k=k, x=x.data_ptr(), ldx=k, w=wq.data_ptr(), ldw=wq.stride(0), sw=ws.data_ptr(), y=y.data_ptr(), ldy=n + 5,
+        d = hip.i8_desc(hip.I8_LINEAR_FIELDS, m=m, n=n, k=k, x=x.data_ptr(), ldx=k, w=wq.data_ptr(), ldw=wq.stride(0), sw=ws.data_ptr(), y=y.data_ptr(), ldy=n + 5,
                          mask=mask.data_ptr(), ldmask=mask.shape[1], q=q.data_ptr(), ldq=k + 40, s=s.data_ptr(), x_type=2, y_type=2, relu=1)
         need = C.c_uint64(0)
-        assert L.dn_i8_linear_workspace(ctx.h, C.byref(d), C.byref(need)) == 0
+        assert L.dn_i8_linear_workspace(ctx.h, d, C.byref(need)) == 0
         ws_ = torch.full((need.value + 512,), 0xA5, dtype=torch.uint8, device="cuda")
         st = torch.cuda.current_stream().cuda_stream
-        assert L.dn_i8_linear(ctx.h, C.byref(d), ws_.data_ptr(), need.value, st) == 0
+        assert L.dn_i8_linear(ctx.h, d, ws_.data_ptr(), need.value, st) == 0
         ref, saved = ctx.i8_linear(x, wq, ws, relu=True, save=True)
         assert torch.equal(y[:m, :n], ref) and (y[:m, n:] == 7).all() and (y[m:] == 7).all()
         assert torch.equal(q[:m, :k], saved.q) and (q[m:] == 77).all() and (q[:m, (k + 15) // 16 * 16:] == 77).all() and not q[:m, k:(k + 15) // 16 * 16].any()
@@ -416,18 +416,18 @@ def test_outputs_end_where_they_end(ctx):
         dx = torch.full((m + 2, k + 3), 7.0, dtype=BF16, device="cuda")
         dw = torch.full((n + 2, k + 3), 7.0, device="cuda")
         db = torch.full((n + 2,), 7.0, device="cuda")
-        g = hip.I8Grad(m=m, n=n, k=k, dy=dy.data_ptr(), ldy=n, mask=mask.data_ptr(), ldmask=mask.shape[1], q=q.data_ptr(), ldq=k + 40, s=s.data_ptr(),
+        g = hip.i8_desc(hip.I8_GRAD_FIELDS, m=m, n=n, k=k, dy=dy.data_ptr(), ldy=n, mask=mask.data_ptr(), ldmask=mask.shape[1], q=q.data_ptr(), ldq=k + 40, s=s.data_ptr(),
                        w=wq.data_ptr(), ldw=wq.stride(0), sw=ws.data_ptr(), dx=dx.data_ptr(), ldx=k + 3, dw=dw.data_ptr(), lddw=k + 3, db=db.data_ptr(), dy_type=2, dw_type=0)
-        assert L.dn_i8_linear_grad_workspace(ctx.h, C.byref(g), C.byref(need)) == 0
+        assert L.dn_i8_linear_grad_workspace(ctx.h, g, C.byref(need)) == 0
         ws_ = torch.full((need.value + 512,), 0xA5, dtype=torch.uint8, device="cuda")
-        assert L.dn_i8_linear_grad(ctx.h, C.byref(g), ws_.data_ptr(), need.value, st) == 0
+        assert L.dn_i8_linear_grad(ctx.h, g, ws_.data_ptr(), need.value, st) == 0
         rx, rw, rb = ctx.i8_linear_grad(dy, saved.q, saved.s, wq, ws, mask=saved.mask, w_dtype=F32)
         assert torch.equal(dx[:m, :k], rx) and (dx[:m, k:] == 7).all() and (dx[m:] == 7).all()
         assert torch.equal(dw[:n, :k], rw) and (dw[:n, k:] == 7).all() and (dw[n:] == 7).all()
         assert torch.equal(db[:n], rb) and (db[n:] == 7).all() and (ws_[need.value:] == 0xA5).all()
         if need.value:
-            assert L.dn_i8_linear_grad(ctx.h, C.byref(g), ws_.data_ptr(), need.value - 1, st) == -3
-            assert L.dn_i8_linear_grad(ctx.h, C.byref(g), ws_.data_ptr() + 8, need.value, st) == -3
+            assert L.dn_i8_linear_grad(ctx.h, g, ws_.data_ptr(), need.value - 1, st) == -3
+            assert L.dn_i8_linear_grad(ctx.h, g, ws_.data_ptr() + 8, need.value, st) == -3
             assert b"workspace" in L.dn_last_error(ctx.h)
 
 
