@@ -50,6 +50,24 @@ template <class T, int N> struct K8Raw {
             }
     }
     __device__ __forceinline__ void load(k8_global p, int have) { load((const T *)(const char *)p, have); }
+    // the largest magnitude; fp32: NaN does not count, 16 bits: it counts as infinity (two magnitudes are compared at a time, as whole numbers)
+    __device__ __forceinline__ float most() const {
+        if constexpr (sizeof(T) == 4) {
+            float m = 0.0f;
+#pragma unroll
+            for (int e = 0; e < N; e++) m = fmaxf(m, fabsf(get(e)));
+            return m;
+        } else {
+            typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+            u2 m = __builtin_bit_cast(u2, w[0] & 0x7fff7fffu);
+#pragma unroll
+            for (unsigned i = 1; i < sizeof w / 4; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u2, w[i] & 0x7fff7fffu));
+            const unsigned t = m[0] > m[1] ? m[0] : m[1];
+            if (t >= (__is_same(T, k8_bf16) ? 0x7f80u : 0x7c00u)) return __uint_as_float(0x7f800000u);
+            K8Raw<T, 2> one = { { t } };
+            return one.get(0);
+        }
+    }
     // the compiler knows nothing of what it computed from these registers before: it forms the values again instead of keeping them
     __device__ __forceinline__ void opaque() {
 #pragma unroll

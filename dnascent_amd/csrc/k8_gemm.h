@@ -5,12 +5,14 @@
 //   tile      BM x BN results per workgroup, WGM x WGN wavefronts, each (BM / WGM) x (BN / WGN) results in 32 x 32 blocks
 //   loads     buffer loads straight into LDS, 16 bytes per lane, two stages; the next step's loads are in flight while this one multiplies.  Rows behind
 //             the matrix and bytes behind the row's end read as zeros (bounds of the buffer descriptor; an offset no buffer has)
-//   LDS       a row's eight 16-byte pieces are stored at piece ^ key(row): eight neighbouring lanes of a fragment read hit eight different pieces
+//   LDS       a row's eight 16-byte pieces are stored at piece ^ (row / 2 & 7): sixteen neighbouring lanes of an operand read (sixteen rows, two to a line of the 64
+//             banks) hit sixteen different places
 //   results   block t of a wavefront holds columns TN c + t (c = lane & 31): a lane's TN blocks are adjacent columns, and a row leaves in runs of
 //             32 TN columns instead of 32
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
@@ -74,20 +76,25 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k8_gemm(G8 g, Epi epi) {
     const char *pa = k8_uniform(g.a + m0 * g.lda), *pb = k8_uniform(g.b + n0 * g.ldb);
     const int per_plane = (g.kb + 127) >> 7, steps = per_plane * g.planes;
     const int s0 = (int)((int64_t)steps * t.z / g.splits), s1 = (int)((int64_t)steps * (t.z + 1) / g.splits);
-    // Load i of a wavefront covers rows 8 (i NW + wave) .. + 7 of the stage, first a's, then b's.  The lane's row and piece (the one that belongs at the LDS place
-    // it writes) are the same in every load of an operand: only the buffer's base moves, and with it how many bytes of the tile are left
+    // Load i of a wavefront covers rows 8 (i NW + wave) .. + 7 of the stage, first a's, then b's; a stage row of b in a block of 64 holds the block's matrix row
+    // 2 c + t at 32 t + c (what a wavefront reads for its block t is then 32 rows in a row).  The lane's row and piece are the same in every load of an operand: only
+    // the buffer's base moves, and with it how many bytes of the tile are left
+    static_assert(TN == 2 && (NW == 4 || NW == 8), "how b's rows are dealt to the loads");
     const int row8 = wave * 8 + (lane >> 3);
-    const int piece_a = ((lane & 7) ^ (row8 & 7)) * 16, piece_b = ((lane & 7) ^ ((row8 / TN) & 7)) * 16;
-    static_assert((8 * NW / TN) % 8 == 0, "b's piece does not depend on the load");
-    const unsigned off_a = (unsigned)(row8 * g.lda) + piece_a, off_b = (unsigned)(row8 * g.ldb) + piece_b;
-    auto fetch = [&](char *l, int s) {
+    const int piece = ((lane & 7) ^ ((row8 >> 1) & 7)) * 16;
+    const unsigned off_a = (unsigned)(row8 * g.lda) + piece, off_b = (unsigned)(((row8 & 31) * 2 + (row8 >> 5)) * g.ldb) + piece;
+    auto fetch = [&](char *l, int s, int from, int to) __attribute__((always_inline)) {        // loads from .. to - 1 of step s
         const int plane = s / per_plane, k = (s - plane * per_plane) << 7;
-        const unsigned oa = k + piece_a < g.kb ? off_a + (unsigned)k : 0x80000000u, ob = k + piece_b < g.kb ? off_b + (unsigned)k : 0x80000000u;
+        const bool any = s >= s0;
+        const bool in = any && k + piece < g.kb;
+        const unsigned oa = in ? off_a + (unsigned)k : 0x80000000u, ob = in ? off_b + (unsigned)k : 0x80000000u;
         const char *at = k8_uniform(pa + plane * g.plane_a);
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
+            if (i < from || i >= to) continue;
             const bool is_a = i * NW * 8 < BM;
-            const unsigned skip = (unsigned)((is_a ? i : i - BM / 8 / NW) * NW * 8) * (unsigned)(is_a ? g.lda : g.ldb), have = is_a ? na : nb;
+            const int ib = i - BM / 8 / NW, rows = is_a ? i * NW * 8 : NW == 8 ? ib * 64 : (ib >> 1) * 64 + (ib & 1);
+            const unsigned skip = (unsigned)rows * (unsigned)(is_a ? g.lda : g.ldb), have = is_a ? na : nb;
             const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)((is_a ? at : pb) + skip), 0, have > skip ? have - skip : 0u, 0x00020000);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(l + (i * NW + wave) * 1024), 16, is_a ? oa : ob, 0, 0, 0);
         }
@@ -100,50 +107,57 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k8_gemm(G8 g, Epi epi) {
 #pragma unroll
             for (int q = 0; q < 16; q++) acc[i][j][q] = 0;
     const int c = lane & 31, h = lane >> 5;
-    const int abase = (wm * TM * 32 + c) * 128, akey = c & 7;
-    const int bbase = (BM + wn * TN * 32 + c * TN) * 128, bkey = c & 7;
-    auto multiply = [&](const char *l, int s) {
-        const int k = (s % per_plane) << 7;
-        const bool tail = I8 && k + 128 > g.kb;
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            i32x4 a[TM], b[TN];
+    const int abase = (wm * TM * 32 + c) * 128, bbase = (BM + wn * TN * 32 + c) * 128, key = (c >> 1) & 7;
+    // LAST: the row may end inside this step.  Integers behind the end: whatever is there counts as zero in one operand, which is enough
+    auto multiply = [&](const char *l, int s, auto last, auto &&next) __attribute__((always_inline)) {
+        i32x4 a[2][TM], b[2][TN];                          // a quarter step's operands are read while the quarter before it multiplies
+        auto operands = [&](int q) __attribute__((always_inline)) {
             const int p = 2 * q + h;
 #pragma unroll
-            for (int i = 0; i < TM; i++) a[i] = *(const i32x4 *)(l + abase + i * 32 * 128 + ((p ^ akey) << 4));
+            for (int i = 0; i < TM; i++) a[q & 1][i] = *(const i32x4 *)(l + abase + i * 32 * 128 + ((p ^ key) << 4));
 #pragma unroll
-            for (int j = 0; j < TN; j++) b[j] = *(const i32x4 *)(l + bbase + j * 128 + ((p ^ bkey) << 4));
-            if (tail) {                                    // integers behind the row's end: whatever is there counts as zero in one operand, which is enough
-                const int left = g.kb - k - p * 16;
+            for (int j = 0; j < TN; j++) b[q & 1][j] = *(const i32x4 *)(l + bbase + j * 32 * 128 + ((p ^ key) << 4));
+        };
+        operands(0);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            if (q < 3) operands(q + 1);
+            next(q);
+            __builtin_amdgcn_sched_barrier(0);
+            if (I8 && decltype(last)::value) {
+                const int left = g.kb - (s << 7) - (2 * q + h) * 16;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int keep = left - 4 * e;
                     const int mask = keep >= 4 ? -1 : keep <= 0 ? 0 : (1 << (8 * keep)) - 1;
 #pragma unroll
-                    for (int i = 0; i < TM; i++) a[i][e] &= mask;
+                    for (int i = 0; i < TM; i++) a[q & 1][i][e] &= mask;
                 }
             }
 #pragma unroll
             for (int i = 0; i < TM; i++)
 #pragma unroll
-                for (int j = 0; j < TN; j++) acc[i][j] = k8_mfma32(a[i], b[j], acc[i][j]);
+                for (int j = 0; j < TN; j++) acc[i][j] = k8_mfma32(a[q & 1][i], b[q & 1][j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    if (s0 < s1) fetch(l0, s0);
-    int s = s0;
+    // steps go in pairs, one left over goes last.  A step that cuts a row of integers has to be that one: the run then starts a step early, on zeros, if it has to
+    const bool cut = I8 && (g.kb & 127) && s1 == steps;
+    int s = s0 - (cut && !((s1 - s0) & 1) ? 1 : 0);
+    // the next step's loads are asked for in the first two quarters of this one: all at once they keep the wavefronts from their products until the queue has taken
+    // them (8192 x 4096 x 4096 in 8 bits: 158.5 us; two quarters 154.9; all four 157.6, the last then land late)
+    constexpr int PER = LOADS / 2;
+    if (s < s1) fetch(l0, s, 0, LOADS);
     for (; s + 1 < s1; s += 2) {
         __syncthreads();                                   // this step's loads have landed, and nobody reads the other stage any more
-        fetch(l1, s + 1);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(l0, s);
+        multiply(l0, s, std::false_type(), [&](int q) __attribute__((always_inline)) { fetch(l1, s + 1, q * PER, min(q * PER + PER, LOADS)); });
         __syncthreads();
-        if (s + 2 < s1) fetch(l0, s + 2);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(l1, s + 1);
+        const bool more = s + 2 < s1;
+        multiply(l1, s + 1, std::false_type(), [&](int q) __attribute__((always_inline)) { if (more) fetch(l0, s + 2, q * PER, min(q * PER + PER, LOADS)); });
     }
     if (s < s1) {
         __syncthreads();
-        multiply(l0, s);
+        multiply(l0, s, std::true_type(), [](int) {});
     }
     // D: column lane & 31, row (q & 3) + 8 (q >> 2) + 4 h.  Lanes outside the matrix stay: an epilogue may put lanes' results together
     const int64_t nn = n0 + wn * TN * 32 + c * TN;

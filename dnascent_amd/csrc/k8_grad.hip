@@ -45,18 +45,19 @@ __device__ __forceinline__ K8Pow k8_pow(unsigned top) {
 }
 
 // ---- dx, narrow layers (N <= 256) ------------------------------------------------------------------------------------------------------------------------------
-// The same shape as the forward pass over narrow rows (k8_narrow): a wavefront takes MT x 16 rows of dy, holds them in registers in the matrix operand's order,
-// finds each row's power of two, and multiplies with the weight, whose transposed fragments lie in LDS as fp16 (256 k x N).  Nothing but dy, the mask and dx
-// moves.  NP: pieces.
-template <class T, int NS, int MT, int NP>
-__global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d) {
+// The same shape as the forward pass over narrow rows (k8_narrow): a wavefront takes 16 rows of dy, holds them in registers in the matrix operand's order, finds
+// each row's power of two, and multiplies with the weight, whose transposed fragments lie in LDS as fp16 (256 k x N).  Nothing but dy, the mask and dx moves.
+// NP: pieces.  WG: threads; the weight fills a CU's LDS where N is 256, and what hides the loads is how many wavefronts the registers leave room for
+template <class T, int NS, int NP, int WG>
+__global__ __launch_bounds__(WG) void k8_dx_narrow(dn_i8_grad_desc d) {
     __shared__ __align__(16) char lw[256 * NS * 64];       // fragment (k block of 64, tile t, step) x 64 lanes x 16 bytes: column k = 64 blk + 4 c + t, n = 32 step + 8 g ..
     __shared__ __align__(16) float lsw[NS * 32];
+    __shared__ __align__(16) unsigned keep[sizeof(T) == 2 ? 256 : 1][4];      // a mask byte as eight 16-bit masks
     const int lane = threadIdx.x & 63, wave = k8_uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int n = (int)d.n;
     const int64_t k0 = (int64_t)blockIdx.y * 256;
     const int cols = (int)min((int64_t)256, d.k - k0), blocks = (cols + 63) / 64;
-    for (int f = threadIdx.x; f < blocks * NS * 64; f += 512) {
+    for (int f = threadIdx.x; f < blocks * NS * 64; f += WG) {
         const int fc = f & 15, fg = (f >> 4) & 3, step = (f >> 6) % NS, blk = (f >> 6) / NS, kk = blk * 64 + 4 * fc;
         unsigned rows[8];
 #pragma unroll
@@ -75,8 +76,17 @@ __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d) {
 #pragma unroll
         for (int t = 0; t < 4; t++) *(i32x4 *)(lw + (((blk * 4 + t) * NS + step) * 64 + fg * 16 + fc) * 16) = out[t];
     }
-    for (int i = threadIdx.x; i < NS * 32; i += 512) lsw[i] = i < n ? d.sw[i] : 0.0f;
+    for (int i = threadIdx.x; i < NS * 32; i += WG) lsw[i] = i < n ? d.sw[i] : 0.0f;
+    if (sizeof(T) == 2 && threadIdx.x < 256)
+#pragma unroll
+        for (int p = 0; p < 4; p++) keep[threadIdx.x][p] = (threadIdx.x >> 2 * p & 1 ? 0xffffu : 0u) | (threadIdx.x >> 2 * p & 2 ? 0xffff0000u : 0u);
     __syncthreads();
+    // A row's power of two comes from max |dz| max |sw| -- an upper bound of its dz sw that needs no products -- unless the channels' scales are more than 2^10 apart:
+    // then, and where something is not finite, from the finite dz sw themselves
+    float swmost = 0.0f, swleast = 0x1.fffffep127f;
+    for (int i = lane; i < n; i += 64) { const float v = fabsf(lsw[i]); swmost = fmaxf(swmost, v); if (v > 0.0f) swleast = fminf(swleast, v); }
+    for (int o = 32; o; o >>= 1) { swmost = fmaxf(swmost, __shfl_xor(swmost, o)); swleast = fminf(swleast, __shfl_xor(swleast, o)); }
+    const bool apart = !(swmost <= swleast * 1024.0f);
     // a lane's places behind a row's end hold no number: `real` has a bit for each that does (byte s of the pair: step s)
     unsigned real[2] = { 0u, 0u };
 #pragma unroll
@@ -84,139 +94,123 @@ __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d) {
         const int have = min(max(n - (s * 32 + 8 * g), 0), 8);
         real[s / 4] |= ((1u << have) - 1u) << (8 * (s % 4));
     }
-    K8Raw<T, 8> raw[MT][NS];
-    unsigned bit[MT][NS];
+    K8Raw<T, 8> raw[NS];
+    unsigned bit[NS];
     const bool masked = d.mask != nullptr;
     // WHOLE: seven more rows lie behind the tile, so that eight numbers can be read at once wherever a row ends (and a lane that has none there reads its row's first)
     auto fetch = [&](int64_t tile, auto kind) __attribute__((always_inline)) {
         constexpr bool WHOLE = decltype(kind)::value;
+        const int64_t first = tile * 16;
+        const unsigned r = WHOLE ? (unsigned)c : (unsigned)min((int64_t)c, d.m - 1 - first);
+        const k8_global p = k8_base((const char *)d.dy + first * d.ldy * (int64_t)sizeof(T));
+        const unsigned row = r * (unsigned)d.ldy * (unsigned)sizeof(T);
 #pragma unroll
-        for (int i = 0; i < MT; i++) {
-            const int64_t first = (tile * MT + i) * 16;
-            const unsigned r = WHOLE ? (unsigned)c : (unsigned)min((int64_t)c, max(d.m - 1 - first, (int64_t)0));
-            const int64_t at0 = WHOLE ? first : min(first, d.m - 1);
-            const k8_global p = k8_base((const char *)d.dy + at0 * d.ldy * (int64_t)sizeof(T));
-            const unsigned row = r * (unsigned)d.ldy * (unsigned)sizeof(T);
+        for (int s = 0; s < NS; s++) {
+            const int at = s * 32 + 8 * g;
+            if (WHOLE) raw[s].load(p + (row + (unsigned)((at < n ? at : 0) * (int)sizeof(T))));
+            else raw[s].load(p + (row + (unsigned)(at * (int)sizeof(T))), n - at);
+        }
+        if (masked) {
+            const k8_global pm = k8_base(d.mask + first * d.ldmask);
 #pragma unroll
             for (int s = 0; s < NS; s++) {
-                const int at = s * 32 + 8 * g;
-                if (WHOLE) raw[i][s].load(p + (row + (unsigned)((at < n ? at : 0) * (int)sizeof(T))));
-                else raw[i][s].load(p + (row + (unsigned)(at * (int)sizeof(T))), n - at);
-            }
-            if (masked) {
-                const k8_global pm = k8_base(d.mask + at0 * d.ldmask);
-#pragma unroll
-                for (int s = 0; s < NS; s++) {
-                    const int at = (s * 32 + 8 * g) >> 3;
-                    bit[i][s] = *(const __attribute__((address_space(1))) unsigned char *)(pm + (r * (unsigned)d.ldmask + (unsigned)(at * 8 < n ? at : 0)));
-                }
+                const int at = (s * 32 + 8 * g) >> 3;
+                bit[s] = *(const __attribute__((address_space(1))) unsigned char *)(pm + (r * (unsigned)d.ldmask + (unsigned)(at * 8 < n ? at : 0)));
             }
         }
     };
     auto work = [&](int64_t tile, auto &&next) __attribute__((always_inline)) {
-        i32x4 a[MT][NP][NS];
-        float down[MT];
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
-            unsigned kept[NS];
+        i32x4 a[NP][NS];
+        // masked numbers and places behind the row's end become zeros, in place
+        if (masked || n != NS * 32)
 #pragma unroll
             for (int s = 0; s < NS; s++) {
-                kept[s] = real[s / 4] >> (8 * (s % 4));
-                if (masked) kept[s] &= bit[i][s];
+                unsigned kept = real[s / 4] >> (8 * (s % 4)) & 255u;
+                if (masked) kept &= bit[s];
+                if constexpr (sizeof(T) == 2) {
+                    const i32x4 m = *(const i32x4 *)keep[kept];
+#pragma unroll
+                    for (int p = 0; p < 4; p++) raw[s].w[p] &= (unsigned)m[p];
+                } else
+#pragma unroll
+                    for (int e = 0; e < 8; e++) raw[s].w[e] &= (unsigned)((int)(kept << (31 - e)) >> 31);
             }
-            // the row's largest dz sw, then the pieces under its power of two.  (dz sw is formed twice: the products are cheaper than the registers.)
-            auto value = [&](int s, int e, const K8Vec<float, 8> &sw) __attribute__((always_inline)) {
-                return __uint_as_float(__float_as_uint(raw[i][s].get(e)) & (unsigned)((int)(kept[s] << (31 - e)) >> 31)) * sw.v[e];
-            };
-            unsigned here = 8 * g;                         // hidden: the 64 factors are read again for every tile instead of being kept
-            k8_opaque(here);
-            float most = 0.0f;                             // (the larger of a number and NaN is the number)
+        auto value = [&](int s, int e, const K8Vec<float, 8> &sw) __attribute__((always_inline)) { return raw[s].get(e) * sw.v[e]; };
+        unsigned here = 8 * g;                             // hidden: the 64 factors are read again for every tile instead of being kept
+        k8_opaque(here);
+        float most = raw[0].most();
+#pragma unroll
+        for (int s = 1; s < NS; s++) most = fmaxf(most, raw[s].most());             // (of 16-bit numbers: NaN counts as infinity)
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        if (apart || __any(!(most <= 0x1.fffffep127f))) {
+            most = 0.0f;
 #pragma unroll
             for (int s = 0; s < NS; s++) {
                 const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + here);
+                raw[s].opaque();
 #pragma unroll
-                for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(value(s, e, sw)));
+                for (int e = 0; e < 8; e++) { const float v = fabsf(value(s, e, sw)); most = fmaxf(most, v <= 0x1.fffffep127f ? v : 0.0f); }
             }
             most = fmaxf(most, __shfl_xor(most, 16));
             most = fmaxf(most, __shfl_xor(most, 32));
-            if (__any(most > 0x1.fffffep127f)) {           // infinite: the power of two comes from the finite ones
-                most = 0.0f;
+        } else most = fminf(most * swmost, 0x1.fffffep127f);
+        const K8Pow pw = k8_pow(__float_as_uint(most));
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int s = 0; s < NS; s++) {
-                    const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + here);
-                    raw[i][s].opaque(); k8_opaque(kept[s]);
+        for (int s = 0; s < NS; s++) {
+            raw[s].opaque(); k8_opaque(here);
+            const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + here);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) { const float v = fabsf(value(s, e, sw)); most = fmaxf(most, v <= 0x1.fffffep127f ? v : 0.0f); }
-                }
-                most = fmaxf(most, __shfl_xor(most, 16));
-                most = fmaxf(most, __shfl_xor(most, 32));
+            for (int p = 0; p < 4; p++) {
+                const float v0 = value(s, 2 * p, sw) * pw.up, v1 = value(s, 2 * p + 1, sw) * pw.up;
+                if (NP == 2) {
+                    const K8Split w = k8_split(v0, v1);
+                    a[0][s][p] = w.hi; a[NP - 1][s][p] = w.lo;
+                } else a[0][s][p] = k8_pack(v0, v1);
             }
-            const K8Pow pw = k8_pow(__float_as_uint(most));
-            down[i] = pw.down;
-            __builtin_amdgcn_sched_barrier(0);
-            // the second pass forms the products again from these registers: 64 of them kept as fp32 do not fit beside the rest
+            // made here and now: sunk behind the next tile's loads, they would keep this tile's numbers alive beside those
 #pragma unroll
-            for (int s = 0; s < NS; s++) {
-                raw[i][s].opaque(); k8_opaque(kept[s]); k8_opaque(here);
-                const K8Vec<float, 8> sw = *(const K8Vec<float, 8> *)(lsw + s * 32 + here);
-#pragma unroll
-                for (int p = 0; p < 4; p++) {
-                    const float v0 = value(s, 2 * p, sw) * pw.up, v1 = value(s, 2 * p + 1, sw) * pw.up;
-                    if (NP == 2) {
-                        const K8Split w = k8_split(v0, v1);
-                        a[i][0][s][p] = w.hi; a[i][NP - 1][s][p] = w.lo;
-                    } else a[i][0][s][p] = k8_pack(v0, v1);
-                }
-                // made here and now: sunk behind the next tile's loads, they would keep this tile's numbers alive beside those
-#pragma unroll
-                for (int p = 0; p < NP; p++) asm volatile("" : "+v"(a[i][p][s]));
-            }
-            __builtin_amdgcn_sched_barrier(0);
+            for (int p = 0; p < NP; p++) asm volatile("" : "+v"(a[p][s]));
         }
+        __builtin_amdgcn_sched_barrier(0);
         next();
         __builtin_amdgcn_sched_barrier(0);
-        float rs[MT][4];
+        float rs[4];
 #pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) rs[i][q] = __shfl(down[i], 4 * g + q);
+        for (int q = 0; q < 4; q++) rs[q] = __shfl(pw.down, 4 * g + q);
         for (int blk = 0; blk < blocks; blk++) {
-            k8_f32x4 acc[MT][4];
+            k8_f32x4 acc[4];
             const char *lb = lw + (blk * 4 * NS * 64 + lane) * 16;
 #pragma unroll
             for (int t = 0; t < 4; t++) {
-#pragma unroll
-                for (int i = 0; i < MT; i++) acc[i][t] = k8_f32x4{ 0, 0, 0, 0 };
+                acc[t] = k8_f32x4{ 0, 0, 0, 0 };
 #pragma unroll
                 for (int s = 0; s < NS; s++) {
                     const i32x4 b = *(const i32x4 *)(lb + (t * NS + s) * 1024);
 #pragma unroll
-                    for (int i = 0; i < MT; i++)
-#pragma unroll
-                        for (int p = 0; p < NP; p++) acc[i][t] = k8_mfma16(a[i][p][s], b, acc[i][t]);
+                    for (int p = 0; p < NP; p++) acc[t] = k8_mfma16(a[p][s], b, acc[t]);
                 }
-                __builtin_amdgcn_sched_barrier(0);         // a tile's fragments at a time: more of them in flight spill
+                __builtin_amdgcn_sched_barrier(0);         // a tile's operands at a time: more of them in flight spill
             }
             const int64_t kk = k0 + blk * 64 + 4 * c;
 #pragma unroll
-            for (int i = 0; i < MT; i++)
+            for (int q = 0; q < 4; q++) {
+                const int64_t mm = tile * 16 + 4 * g + q;
+                if (mm >= d.m || kk >= d.k) continue;
+                T *p = (T *)d.dx + mm * d.ldx + kk;
+                K8Vec<T, 4> o;
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int64_t mm = (tile * MT + i) * 16 + 4 * g + q;
-                    if (mm >= d.m || kk >= d.k) continue;
-                    T *p = (T *)d.dx + mm * d.ldx + kk;
-                    K8Vec<T, 4> o;
+                for (int t = 0; t < 4; t++) o.v[t] = (T)(acc[t][q] * rs[q]);
+                if (kk + 4 <= d.k) k8_stream<T, 4>(p, o);
+                else
 #pragma unroll
-                    for (int t = 0; t < 4; t++) o.v[t] = (T)(acc[i][t][q] * rs[i][q]);
-                    if (kk + 4 <= d.k) k8_store<T, 4>(p, o);
-                    else
-#pragma unroll
-                        for (int t = 0; t < 4; t++) if (kk + t < d.k) p[t] = o.v[t];
-                }
+                    for (int t = 0; t < 4; t++) if (kk + t < d.k) p[t] = o.v[t];
+            }
         }
     };
-    const int64_t tiles = (d.m + 16 * MT - 1) / (16 * MT), stride = (int64_t)gridDim.x * 8, whole = d.ldy ? max(d.m - 7, (int64_t)0) / (16 * MT) : 0;
-    int64_t tile = (int64_t)blockIdx.x * 8 + wave;
+    const int64_t tiles = (d.m + 15) / 16, stride = (int64_t)gridDim.x * (WG / 64), whole = d.ldy ? max(d.m - 7, (int64_t)0) / 16 : 0;
+    int64_t tile = (int64_t)blockIdx.x * (WG / 64) + wave;
     if (tile < whole) fetch(tile, std::true_type());
     for (; tile < whole; tile += stride) work(tile, [&]() __attribute__((always_inline)) { if (tile + stride < whole) fetch(tile + stride, std::true_type()); });
     for (; tile < tiles; tile += stride) {
@@ -355,8 +349,8 @@ __global__ __launch_bounds__(256) void k8_dx_join(const float *__restrict__ part
 // sees one that does not fit raises a flag; behind the barrier the workgroup then finds the tile's largest numbers, lowers the powers of the channels that need
 // it (five bits of room), scales their sums so far -- exactly -- and makes the tile again.  That happens for a workgroup's first tile and hardly ever after.
 //
-// LDS row of a channel: RT rows x 2 bytes (x NP pieces), in pieces of 16 bytes at piece ^ ((channel >> 2) & 7): threads that write and lanes that read four channels
-// apart hit different banks.  Wavefronts share the S x S results in blocks of 64 x KB; where there are fewer blocks than wavefronts, sets of wavefronts take turns
+// LDS row of a channel: RT rows x 2 bytes (x NP pieces), in pieces of 16 bytes.  Threads that write and lanes that read stand four channels apart: those lie side by side, and
+// sixteen of them reach sixteen different places of the 64 banks.  Wavefronts share the S x S results in blocks of 64 x KB; where there are fewer blocks than wavefronts, sets of wavefronts take turns
 // with the steps of 32 rows and join their sums at the end.
 template <int S, int NP> struct DwShape {
     static constexpr int RT = 16384 / S / NP;              // rows of a tile: S = 256: 64, 128: 128, 64: 256 (half with two pieces)
@@ -364,6 +358,9 @@ template <int S, int NP> struct DwShape {
     static constexpr int UROW = RT * 2 * NP, QROW = RT * 2; // bytes of a channel's row
     static constexpr int LDS = S * (UROW + QROW);           // one stage
 };
+template <int ROW> __device__ __forceinline__ int k8_place(int block, int i, int c, int piece) {      // channel 64 block + 4 c + i; ROW: bytes of a channel's row
+    return (block * 64 + i * 16 + c) * ROW + ((piece ^ (ROW >= 256 ? c : ROW == 128 ? c >> 1 : c >> 2)) << 4);
+}
 struct DwOut { float *part, *part_b; int splits, tiles_n, tiles_k; int64_t run; };   // part [splits][n][k], part_b [splits][n]; run: rows of a split, a multiple of RT
 
 template <class W> __device__ __forceinline__ void k8_put4(W *p, const float (&v)[4], int64_t left) {
@@ -462,27 +459,33 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
                 else if (!d.mask) rbit[e] = ch < ncols ? 255u : 0u;
     };
     float pw[4] = { 0x1p126f, 0x1p126f, 0x1p126f, 0x1p126f }, sum[4] = { 0, 0, 0, 0 };
-    auto dz = [&](int e, int j) { return rbit[e] >> (esh + j) & 1 ? raw[e].get(j) : 0.0f; };
-    // the turned fp16 values of this thread's task (and, the first time, the sums of dz); true if one does not fit
-    auto make = [&](char *l, auto first) __attribute__((always_inline)) {
+    auto dz = [&](int e, int j) { return __uint_as_float(__float_as_uint(raw[e].get(j)) & (unsigned)((int)(rbit[e] << (31 - j)) >> 31)); };       // rbit: from this thread's first channel on
+    // the turned fp16 values of this thread's task (and, if asked for, the sums of dz); true if one does not fit
+    auto make = [&](char *l, auto masked, auto sums) __attribute__((always_inline)) {
         float most = 0.0f;
-        if (has_u)
+        if (has_u) {
+            if (decltype(masked)::value)
+#pragma unroll
+                for (int e = 0; e < 8; e++) rbit[e] >>= esh;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 i32x4 hi, lo;
 #pragma unroll
                 for (int p = 0; p < 4; p++) {
-                    const float z0 = dz(2 * p, j), z1 = dz(2 * p + 1, j), v0 = z0 * rs[2 * p] * pw[j], v1 = z1 * rs[2 * p + 1] * pw[j];
-                    if (decltype(first)::value) sum[j] = sum[j] + z0 + z1;
-                    most = fmaxf(most, fmaxf(fabsf(v0), fabsf(v1)));
+                    const float z0 = decltype(masked)::value ? dz(2 * p, j) : raw[2 * p].get(j), z1 = decltype(masked)::value ? dz(2 * p + 1, j) : raw[2 * p + 1].get(j);
+                    const float v0 = z0 * rs[2 * p] * pw[j], v1 = z1 * rs[2 * p + 1] * pw[j];
+                    if (decltype(sums)::value) sum[j] = sum[j] + z0 + z1;
+                    most = fmaxf(fmaxf(fabsf(v0), fabsf(v1)), most);
                     if (NP == 2) { const K8Split w = k8_split(v0, v1); hi[p] = w.hi; lo[p] = w.lo; }
                     else hi[p] = k8_pack(v0, v1);
                 }
-                const int key = ((ch + j) >> 2) & 7;
-                char *row = l + (ch + j) * D::UROW;
-                *(i32x4 *)(row + ((rg ^ key) << 4)) = hi;
-                if (NP == 2) *(i32x4 *)(row + (((rg + D::RT / 8) ^ key) << 4)) = lo;
+                *(i32x4 *)(l + k8_place<D::UROW>(ch >> 6, j, ch >> 2 & 15, rg)) = hi;
+                if (NP == 2) *(i32x4 *)(l + k8_place<D::UROW>(ch >> 6, j, ch >> 2 & 15, rg + D::RT / 8)) = lo;
             }
+            if (decltype(masked)::value)
+#pragma unroll
+                for (int e = 0; e < 8; e++) rbit[e] <<= esh;
+        }
         return most > 32768.0f;
     };
     auto make_q = [&](char *l) __attribute__((always_inline)) {
@@ -490,7 +493,7 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
         i32x4 out[4];
         k8_columns(rq, out);
 #pragma unroll
-        for (int j = 0; j < 4; j++) *(i32x4 *)(l + S * D::UROW + (ch + j) * D::QROW + ((rg ^ (((ch + j) >> 2) & (D::QROW >= 128 ? 7 : 3))) << 4)) = out[j];
+        for (int j = 0; j < 4; j++) *(i32x4 *)(l + S * D::UROW + k8_place<D::QROW>(ch >> 6, j, ch >> 2 & 15, rg)) = out[j];
     };
     const int block = wave % D::BLOCKS, set = wave / D::BLOCKS, bn = block % (S / 64), bk = block / (S / 64);
     constexpr int TK = D::KB / 16;
@@ -499,7 +502,7 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < TK; j++) acc[i][j] = k8_f32x4{ 0, 0, 0, 0 };
-    // tile i of a block of 64 holds channels 4 c + i: key = c & 7
+    // tile i of a block of 64 holds channels 4 c + i
     auto multiply = [&](const char *l) __attribute__((always_inline)) {
 #pragma unroll
         for (int w = 0; w < (D::STEPS * NP + D::SETS - 1) / D::SETS; w++) {
@@ -507,10 +510,10 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
             if (D::STEPS * NP % D::SETS && item >= D::STEPS * NP) break;
             i32x4 a[4], b[TK];
 #pragma unroll
-            for (int i = 0; i < 4; i++) a[i] = *(const i32x4 *)(l + (bn * 64 + 4 * c + i) * D::UROW + (((plane * (D::RT / 8) + step * 4 + g) ^ (c & 7)) << 4));
+            for (int i = 0; i < 4; i++) a[i] = *(const i32x4 *)(l + k8_place<D::UROW>(bn, i, c, plane * (D::RT / 8) + step * 4 + g));
 #pragma unroll
             for (int j = 0; j < TK; j++)
-                b[j] = *(const i32x4 *)(l + S * D::UROW + (bk * D::KB + (j / 4) * 64 + 4 * c + j % 4) * D::QROW + (((step * 4 + g) ^ (c & (D::QROW >= 128 ? 7 : 3))) << 4));
+                b[j] = *(const i32x4 *)(l + S * D::UROW + k8_place<D::QROW>(bk * (D::KB / 64) + j / 4, j % 4, c, step * 4 + g));
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -518,16 +521,20 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
         }
     };
     int stage = 0;
-    auto tile = [&](auto &&next) __attribute__((always_inline)) {
+    // again, next: fetch this tile / the next one
+    auto tile = [&](auto whole, auto &&again, auto &&next) __attribute__((always_inline)) {
         char *l = lds[stage];
-        const bool over = make(l, std::true_type());
+        bool over;
+        if (!decltype(whole)::value) over = make(l, std::true_type(), std::true_type());
+        else if (d.mask) over = with_b ? make(l, std::true_type(), std::true_type()) : make(l, std::true_type(), std::false_type());
+        else over = with_b ? make(l, std::false_type(), std::true_type()) : make(l, std::false_type(), std::false_type());
         if (with_q) {
             make_q(l);
             if (over) raised[stage] = 1;                   // (any lane; all that write write 1)
+            next();
             __syncthreads();
             if (raised[stage]) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) raw[e].opaque();
+                again();
                 for (int i = tid; i < S; i += 512) peak[i] = 0u;
                 __syncthreads();
                 if (has_u)
@@ -535,7 +542,7 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
                     for (int j = 0; j < 4; j++) {
                         unsigned top = 0;
 #pragma unroll
-                        for (int e = 0; e < 8; e++) { const unsigned v = k8_mag(dz(e, j) * rs[e]); top = max(top, v < 0x7f800000u ? v : 0u); }
+                        for (int e = 0; e < 8; e++) { const unsigned v = k8_mag((rbit[e] >> (esh + j) & 1 ? raw[e].get(j) : 0.0f) * rs[e]); top = max(top, v < 0x7f800000u ? v : 0u); }
                         atomicMax(&peak[ch + j], top);
                     }
                 __syncthreads();
@@ -560,22 +567,23 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
                     }
 #pragma unroll
                 for (int e = 0; e < 8; e++) raw[e].opaque();
-                (void)make(l, std::false_type());
+                (void)make(l, std::true_type(), std::false_type());
+                next();
                 __syncthreads();
             }
-        }
-        next();
-        if (with_q) multiply(l);
+            multiply(l);
+        } else next();
         stage ^= 1;
     };
     // (a call without rows has one empty run: its sums are zeros)
     int64_t base = r0;
     const int64_t whole = min(r1, d.ldy && d.ldq ? d.m - 3 : (int64_t)0) - D::RT;         // the last tile that can be fetched whole starts here or before
     if (base <= whole) fetch(base, std::true_type());
-    for (; base <= whole; base += D::RT) tile([&]() __attribute__((always_inline)) { if (base + D::RT <= whole) fetch(base + D::RT, std::true_type()); });
+    for (; base <= whole; base += D::RT) tile(std::true_type(), [&]() __attribute__((always_inline)) { fetch(base, std::true_type()); },
+                                                        [&]() __attribute__((always_inline)) { if (base + D::RT <= whole) fetch(base + D::RT, std::true_type()); });
     for (; base < r1; base += D::RT) {
         fetch(base, std::false_type());
-        tile([]() {});
+        tile(std::false_type(), [&]() __attribute__((always_inline)) { fetch(base, std::false_type()); }, []() {});
     }
     // ---- the sums leave: sets of wavefronts joined in LDS first, in the order of the sets
     __syncthreads();
@@ -725,12 +733,12 @@ template <class T, int NP, class Epi> hipError_t dx_gemm(const dn_i8_grad_desc &
 }
 template <class T, int NP> hipError_t dx_of(const dn_i8_grad_desc &d, const Plan &p, char *base, hipStream_t st) {
     if (p.narrow) {
-        constexpr int MT = NP == 1 ? 2 : 1;
         const unsigned per = (unsigned)((d.k + 255) / 256);
-        const int64_t wgs = (d.m + 128 * MT - 1) / (128 * MT);
-        if (d.n <= 64) k8_dx_narrow<T, 2, MT, NP><<<dim3((unsigned)std::min<int64_t>(wgs, 2 * K8_CUS / per), per), 512, 0, st>>>(d);
-        else if (d.n <= 128) k8_dx_narrow<T, 4, MT, NP><<<dim3((unsigned)std::min<int64_t>(wgs, 2 * K8_CUS / per), per), 512, 0, st>>>(d);
-        else k8_dx_narrow<T, 8, MT, NP><<<dim3((unsigned)std::min<int64_t>(wgs, K8_CUS / per), per), 512, 0, st>>>(d);
+        auto grid = [&](int wg, int each) { return dim3((unsigned)std::min<int64_t>((d.m + wg / 4 - 1) / (wg / 4), each * K8_CUS / per), per); };      // a wavefront has 16 rows
+        constexpr int WIDEST = NP == 1 ? 768 : 512;
+        if (d.n <= 64) k8_dx_narrow<T, 2, NP, 512><<<grid(512, 4), 512, 0, st>>>(d);
+        else if (d.n <= 128) k8_dx_narrow<T, 4, NP, 512><<<grid(512, 2), 512, 0, st>>>(d);
+        else k8_dx_narrow<T, 8, NP, WIDEST><<<grid(WIDEST, 1), WIDEST, 0, st>>>(d);
         return hipGetLastError();
     }
     _Float16 *pieces = (_Float16 *)(base + p.pieces), *turned = (_Float16 *)(base + p.turned);
