@@ -174,20 +174,19 @@ struct Out {                                               // the epilogue's hal
 __device__ __forceinline__ float k8_finish(int acc, float sw, float sx, float bias) {
     return (float)acc * sw * sx + bias;                    // the row's scale last: a row near fp32's end overflows only if its result does
 }
-// TN adjacent columns of one row.  The mask's bits: the 32 lanes of a half wavefront hold 32 TN adjacent columns of the row; lanes put their TN bits together
-// into bytes (the columns of a half start at a multiple of 32 TN, so bytes never straddle halves)
+// TN adjacent columns of one row: what is added to them, and where they go
 template <class T, int TN>
-__device__ __forceinline__ void k8_put(const Out &o, int64_t mm, int64_t nn, float (&v)[TN]) {
-    if (o.residual) {
-        const T *r = (const T *)o.residual + mm * o.ldr + nn;
-        if (nn + TN <= o.n) {
-            const K8Vec<T, TN> t = k8_load<T, TN>(r);
+__device__ __forceinline__ K8Vec<T, TN> k8_added(const Out &o, int64_t mm, int64_t nn) {
+    K8Vec<T, TN> t;
+    const T *r = (const T *)o.residual + mm * o.ldr + nn;
+    if (nn + TN <= o.n) t = k8_load<T, TN>(r);
+    else
 #pragma unroll
-            for (int j = 0; j < TN; j++) v[j] += (float)t.v[j];
-        } else
-#pragma unroll
-            for (int j = 0; j < TN; j++) if (nn + j < o.n) v[j] += (float)r[j];
-    }
+        for (int j = 0; j < TN; j++) t.v[j] = nn + j < o.n ? r[j] : (T)0.0f;
+    return t;
+}
+template <class T, int TN>
+__device__ __forceinline__ void k8_put(const Out &o, int64_t mm, int64_t nn, const float (&v)[TN]) {
     K8Vec<T, TN> y;
 #pragma unroll
     for (int j = 0; j < TN; j++) y.v[j] = (T)(o.relu ? k8_relu(v[j]) : v[j]);
@@ -197,6 +196,8 @@ __device__ __forceinline__ void k8_put(const Out &o, int64_t mm, int64_t nn, flo
 #pragma unroll
         for (int j = 0; j < TN; j++) if (nn + j < o.n) p[j] = y.v[j];
 }
+// The mask's bits: the 32 lanes of a half wavefront hold 32 TN adjacent columns of a row; lanes put their TN bits together into bytes (the columns of a half start
+// at a multiple of 32 TN, so bytes never straddle halves)
 template <int TN>
 __device__ __forceinline__ void k8_put_mask(const Out &o, int64_t mm, int64_t nn, const float (&v)[TN], bool live) {
     // every lane of the wavefront comes here; 8 / TN neighbouring lanes share a byte
@@ -220,11 +221,20 @@ struct LinearEpi {
         for (int j = 0; j < TN; j++) { const int64_t n = min(nn + j, o.n - 1); c.sw[j] = o.sw[n]; c.bias[j] = o.bias ? o.bias[n] : 0.0f; }
         return c;
     }
-    __device__ __forceinline__ float row(int64_t mm) const { return o.sx[mm]; }
-    template <int TN> __device__ __forceinline__ void store(const Columns<TN> &c, float sx, int64_t mm, int64_t nn, int, const int (&acc)[TN], bool live) const {
+    template <int TN> struct Row { float sx; K8Vec<T, TN> added; };
+    template <int TN> __device__ __forceinline__ Row<TN> row(int64_t mm, int64_t nn) const {
+        Row<TN> r;
+        r.sx = o.sx[mm];
+        if (o.residual) r.added = k8_added<T, TN>(o, mm, nn);
+        return r;
+    }
+    template <int TN> __device__ __forceinline__ void store(const Columns<TN> &c, const Row<TN> &r, int64_t mm, int64_t nn, int, const int (&acc)[TN], bool live) const {
         float v[TN];
 #pragma unroll
-        for (int j = 0; j < TN; j++) v[j] = k8_finish(acc[j], c.sw[j], sx, c.bias[j]);
+        for (int j = 0; j < TN; j++) v[j] = k8_finish(acc[j], c.sw[j], r.sx, c.bias[j]);
+        if (o.residual)
+#pragma unroll
+            for (int j = 0; j < TN; j++) v[j] += (float)r.added.v[j];
         if (live) k8_put<T, TN>(o, mm, nn, v);
         if (o.mask) k8_put_mask<TN>(o, mm, nn, v, live);
     }
@@ -235,8 +245,9 @@ struct PartEpi {
     int *part; int64_t m, n;
     template <int TN> struct Columns {};
     template <int TN> __device__ __forceinline__ Columns<TN> columns(int64_t) const { return {}; }
-    __device__ __forceinline__ float row(int64_t) const { return 0.0f; }
-    template <int TN> __device__ __forceinline__ void store(const Columns<TN> &, float, int64_t mm, int64_t nn, int z, const int (&acc)[TN], bool live) const {
+    template <int TN> struct Row {};
+    template <int TN> __device__ __forceinline__ Row<TN> row(int64_t, int64_t) const { return {}; }
+    template <int TN> __device__ __forceinline__ void store(const Columns<TN> &, const Row<TN> &, int64_t mm, int64_t nn, int z, const int (&acc)[TN], bool live) const {
         if (!live) return;
         int *p = part + ((int64_t)z * m + mm) * n + nn;
         K8Vec<int, TN> v;
@@ -257,6 +268,7 @@ __global__ __launch_bounds__(256) void k8_join(const int *__restrict__ part, int
     const bool live = nn < o.n;
     int acc[4] = { 0, 0, 0, 0 };
     if (live)
+#pragma unroll 4
         for (int z = 0; z < splits; z++) {
             const int *p = part + ((int64_t)z * o.m + mm) * o.n + nn;
             if (nn + 4 <= o.n) {
@@ -268,7 +280,7 @@ __global__ __launch_bounds__(256) void k8_join(const int *__restrict__ part, int
                 for (int j = 0; j < 4; j++) if (nn + j < o.n) acc[j] += p[j];
         }
     const LinearEpi<T> e{ o };
-    e.template store<4>(e.template columns<4>(live ? nn : 0), o.sx[mm], mm, nn, 0, acc, live);
+    e.template store<4>(e.template columns<4>(live ? nn : 0), e.template row<4>(mm, live ? nn : 0), mm, nn, 0, acc, live);
 }
 
 // rows at a pitch the product cannot fetch (not a multiple of 16 bytes), copied to one that it can, zeros behind their ends
@@ -406,10 +418,15 @@ __global__ __launch_bounds__(512) void k8_few(const X *__restrict__ x, int64_t l
         const int64_t nn = n0 + (i & 15), nc = min(nn, o.n - 1);
         const bool live = r < m && nn < o.n;
         float v[1] = { k8_finish(a, o.sw[nc], scales[min(r, m - 1)], o.bias ? o.bias[nc] : 0.0f) };
+        auto put = [&](auto one) __attribute__((always_inline)) {
+            typedef decltype(one) Y;
+            if (o.residual) v[0] += (float)k8_added<Y, 1>(o, r, nn).v[0];
+            k8_put<Y, 1>(o, r, nn, v);
+        };
         if (live) {
-            if (y_type == DN_T_F32) k8_put<float, 1>(o, r, nn, v);
-            else if (y_type == DN_T_F16) k8_put<_Float16, 1>(o, r, nn, v);
-            else k8_put<k8_bf16, 1>(o, r, nn, v);
+            if (y_type == DN_T_F32) put(0.0f);
+            else if (y_type == DN_T_F16) put((_Float16)0.0f);
+            else put((k8_bf16)0.0f);
         }
         if (o.mask) k8_put_mask<1>(o, r, nn, v, live);
     }
@@ -530,12 +547,19 @@ __global__ __launch_bounds__(512) void k8_narrow(const X *__restrict__ x, int64_
             }
             const k8_f32x4 sw = *(const k8_f32x4 *)(lsw + blk * 64 + 4 * c), bias = *(const k8_f32x4 *)(lbias + blk * 64 + 4 * c);
             const int64_t nn = n0 + blk * 64 + 4 * c;
+            K8Vec<Y, 4> added[4];
+            if (o.residual)
+#pragma unroll
+                for (int i = 0; i < 4; i++) added[i] = k8_added<Y, 4>(o, min(tile * 16 + 4 * g + i, o.m - 1), nn);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int64_t mm = tile * 16 + 4 * g + i;
                 float v[4];
 #pragma unroll
                 for (int t = 0; t < 4; t++) v[t] = k8_finish(acc[t][i], sw[t], rs[i], bias[t]);
+                if (o.residual)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) v[t] += (float)added[i].v[t];
                 const bool live = mm < o.m && nn < o.n;
                 if (live) k8_put<Y, 4>(o, mm, nn, v);
                 if (o.mask) k8_put_mask<4>(o, mm, nn, v, live);
@@ -569,7 +593,7 @@ Plan plan_linear(const dn_i8_linear_desc &d) {
     if (given ? !k8_direct(d.x, d.ldx) : d.q && !k8_direct(d.q, d.ldq)) p.x = take((uint64_t)d.m * k8_up(d.k, 16));
     if (!k8_direct(d.w, d.ldw)) p.w = take((uint64_t)d.n * k8_up(d.k, 16));
     const int64_t t256 = ((d.m + 255) / 256) * ((d.n + 255) / 256), t128 = ((d.m + 127) / 128) * ((d.n + 127) / 128), steps = (d.k + 127) / 128;
-    p.big = t256 >= K8_CUS;
+    p.big = t256 >= K8_CUS && d.n > 64;
     if (!p.big && t128 < K8_CUS) {                         // fewer tiles than compute units: the reduction is cut, four steps at least to a run
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(K8_CUS / t128, steps / 4));
         if (p.splits > 1) p.part = take((uint64_t)p.splits * d.m * d.n * 4);
@@ -578,10 +602,12 @@ Plan plan_linear(const dn_i8_linear_desc &d) {
 }
 
 template <class Epi> hipError_t gemm_i8(G8 g, bool big, const Epi &e, hipStream_t st) {
-    const int b = big ? 256 : 128;
-    g.tiles_m = (int)((g.m + b - 1) / b); g.tiles_n = (int)((g.n + b - 1) / b);
+    const bool slim = g.n <= 64;
+    const int bm = big ? 256 : 128, bn = big ? 256 : slim ? 64 : 128;
+    g.tiles_m = (int)((g.m + bm - 1) / bm); g.tiles_n = (int)((g.n + bn - 1) / bn);
     const unsigned grid = (unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits);
-    if (big) k8_gemm<true, 256, 256, 2, 4, Epi><<<dim3(grid), 512, 0, st>>>(g, e);
+    if (slim) k8_gemm<true, 128, 64, 4, 1, Epi><<<dim3(grid), 256, 0, st>>>(g, e);
+    else if (big) k8_gemm<true, 256, 256, 2, 4, Epi><<<dim3(grid), 512, 0, st>>>(g, e);
     else k8_gemm<true, 128, 128, 2, 2, Epi><<<dim3(grid), 256, 0, st>>>(g, e);
     return hipGetLastError();
 }

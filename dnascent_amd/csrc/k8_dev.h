@@ -29,15 +29,21 @@ template <class T, int N> struct K8Raw {
         else { typedef _Float16 h2 __attribute__((ext_vector_type(2))); return (float)__builtin_bit_cast(h2, w[e / 2])[e & 1]; }
     }
     __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(w, (const K8Vec<T, N> *)p, sizeof w); }
-    __device__ __forceinline__ void load(const T *p, int have) {             // the first `have`, zeros behind them
+    // the first `have`, zeros behind them; p[have - 1] is the row's last number, even if p lies behind it.  No branch: a load in a branch of its own is waited for there
+    __device__ __forceinline__ void load(const T *p, int have) {
+        unsigned v[N];
 #pragma unroll
-        for (unsigned i = 0; i < sizeof w / 4; i++) w[i] = 0u;
+        for (int e = 0; e < N; e++) {
+            if constexpr (sizeof(T) == 4) v[e] = *(const unsigned *)(p + min(e, have - 1));
+            else v[e] = *(const uint16_t *)(p + min(e, have - 1));
+        }
 #pragma unroll
-        for (int e = 0; e < N; e++)
-            if (e < have) {
-                if constexpr (sizeof(T) == 4) w[e] = *(const unsigned *)(p + e);
-                else w[e / 2] |= (unsigned)*(const uint16_t *)(p + e) << (16 * (e & 1));
-            }
+        for (int e = 0; e < N; e++) v[e] = e < have ? v[e] : 0u;
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof w / 4); i++) {
+            if constexpr (sizeof(T) == 4) w[i] = v[i];
+            else w[i] = v[2 * i] | v[2 * i + 1] << 16;
+        }
     }
     __device__ __forceinline__ void load(k8_global p) {
         if constexpr (sizeof w == 8) { const k8_u32x2 v = *(const __attribute__((address_space(1))) k8_u32x2 *)p; w[0] = v[0]; w[1] = v[1]; }

@@ -59,7 +59,7 @@ __device__ __forceinline__ K8Tile k8_tile(const G8 &g, int bid, int total) {
     return { first + r % size, r / size, z };
 }
 
-// The epilogue: columns(first column of a lane), row(row), store(those, row, column, run z, values of TN adjacent columns, whether the row and column exist)
+// The epilogue: columns(a lane's first column), row(row, column), store(those, row, column, run z, values of TN adjacent columns, whether the row and column exist)
 template <bool I8, int BM, int BN, int WGM, int WGN, class Epi>
 __global__ __launch_bounds__(64 * WGM * WGN) void k8_gemm(G8 g, Epi epi) {
     constexpr int NW = WGM * WGN, TM = BM / WGM / 32, TN = BN / WGN / 32, LOADS = (BM + BN) / 8 / NW;
@@ -159,18 +159,25 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k8_gemm(G8 g, Epi epi) {
         __syncthreads();
         multiply(l0, s, std::true_type(), [](int) {});
     }
-    // D: column lane & 31, row (q & 3) + 8 (q >> 2) + 4 h.  Lanes outside the matrix stay: an epilogue may put lanes' results together
+    // D: column lane & 31, row (q & 3) + 8 (q >> 2) + 4 h.  Lanes outside the matrix stay: an epilogue may put lanes' results together.  What it reads for 16 rows is
+    // asked for before the first of them is finished
     const int64_t nn = n0 + wn * TN * 32 + c * TN;
     const auto cols = epi.template columns<TN>(nn);
 #pragma unroll
-    for (int i = 0; i < TM; i++)
+    for (int i = 0; i < TM; i++) {
+        const int64_t m1 = m0 + wm * TM * 32 + i * 32 + 4 * h;
+        typename Epi::template Row<TN> rows[16];
+#pragma unroll
+        for (int q = 0; q < 16; q++) rows[q] = epi.template row<TN>(min(m1 + (q & 3) + 8 * (q >> 2), g.m - 1), nn);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int q = 0; q < 16; q++) {
-            const int64_t mm = m0 + wm * TM * 32 + i * 32 + (q & 3) + 8 * (q >> 2) + 4 * h;
+            const int64_t mm = m1 + (q & 3) + 8 * (q >> 2);
             typename Epi::value v[TN];
 #pragma unroll
             for (int j = 0; j < TN; j++) v[j] = acc[i][j][q];
-            epi.template store<TN>(cols, epi.row(min(mm, g.m - 1)), mm, nn, t.z, v, mm < g.m && nn < g.n);
+            epi.template store<TN>(cols, rows[q], mm, nn, t.z, v, mm < g.m && nn < g.n);
             if (q % 4 == 3) __builtin_amdgcn_sched_barrier(0);                // a few rows at a time: the registers are full
         }
+    }
 }

@@ -301,14 +301,15 @@ struct DxEpi {
     const float *down; T *dx; int64_t k, ldx;
     template <int TN> struct Columns {};
     template <int TN> __device__ __forceinline__ Columns<TN> columns(int64_t) const { return {}; }
-    __device__ __forceinline__ float row(int64_t mm) const { return down[mm]; }
-    template <int TN> __device__ __forceinline__ void store(const Columns<TN> &, float s, int64_t mm, int64_t kk, int, const float (&acc)[TN], bool live) const {
+    template <int TN> struct Row { float down; };
+    template <int TN> __device__ __forceinline__ Row<TN> row(int64_t mm, int64_t) const { return { down[mm] }; }
+    template <int TN> __device__ __forceinline__ void store(const Columns<TN> &, const Row<TN> &r, int64_t mm, int64_t kk, int, const float (&acc)[TN], bool live) const {
         if (!live) return;
         T *p = dx + mm * ldx + kk;
         K8Vec<T, TN> o;
 #pragma unroll
-        for (int j = 0; j < TN; j++) o.v[j] = (T)(acc[j] * s);
-        if (kk + TN <= k) k8_store<T, TN>(p, o);
+        for (int j = 0; j < TN; j++) o.v[j] = (T)(acc[j] * r.down);
+        if (kk + TN <= k) k8_stream<T, TN>(p, o);
         else
 #pragma unroll
             for (int j = 0; j < TN; j++) if (kk + j < k) p[j] = o.v[j];
@@ -320,8 +321,9 @@ struct DxPart {
     float *part; int64_t m, k;
     template <int TN> struct Columns {};
     template <int TN> __device__ __forceinline__ Columns<TN> columns(int64_t) const { return {}; }
-    __device__ __forceinline__ float row(int64_t) const { return 0.0f; }
-    template <int TN> __device__ __forceinline__ void store(const Columns<TN> &, float, int64_t mm, int64_t kk, int z, const float (&acc)[TN], bool live) const {
+    template <int TN> struct Row {};
+    template <int TN> __device__ __forceinline__ Row<TN> row(int64_t, int64_t) const { return {}; }
+    template <int TN> __device__ __forceinline__ void store(const Columns<TN> &, const Row<TN> &, int64_t mm, int64_t kk, int z, const float (&acc)[TN], bool live) const {
         if (!live) return;
         float *p = part + ((int64_t)z * m + mm) * k + kk;
 #pragma unroll
@@ -332,11 +334,141 @@ template <class T>
 __global__ __launch_bounds__(256) void k8_dx_join(const float *__restrict__ part, int splits, const float *__restrict__ down, T *__restrict__ dx, int64_t m, int64_t k, int64_t ldx) {
     const int64_t kb = (k + 255) / 256, w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (w >= m * kb) return;
-    const int64_t mm = w / kb, kk = (w % kb) * 256 + (threadIdx.x & 63) * 4;
-    for (int j = 0; j < 4 && kk + j < k; j++) {
-        float s = 0.0f;
-        for (int z = 0; z < splits; z++) s += part[((int64_t)z * m + mm) * k + kk + j];
-        dx[mm * ldx + kk + j] = (T)(s * down[mm]);
+    const int64_t mm = w / kb, kk = (w % kb) * 256 + (threadIdx.x & 63) * 4, left = k - kk;
+    if (left <= 0) return;
+    float v[4] = { 0, 0, 0, 0 };
+    const float *p = part + mm * k + kk;
+    if (left >= 4)
+#pragma unroll 8
+        for (int z = 0; z < splits; z++) {
+            const K8Vec<float, 4> t = k8_load<float, 4>(p + (int64_t)z * m * k);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] += t.v[j];
+        }
+    else
+        for (int z = 0; z < splits; z++)
+#pragma unroll
+            for (int j = 0; j < 3; j++) if (j < left) v[j] += p[(int64_t)z * m * k + j];
+    const float s = down ? down[mm] : 1.0f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] *= s;
+    T *o = dx + mm * ldx + kk;
+    K8Vec<T, 4> y;
+#pragma unroll
+    for (int j = 0; j < 4; j++) y.v[j] = (T)v[j];
+    if (left >= 4) k8_store<T, 4>(o, y);
+    else
+#pragma unroll
+        for (int j = 0; j < 3; j++) if (j < left) o[j] = y.v[j];
+}
+
+// ---- dx, few rows (M <= 16): the weight is streamed once, turned in registers -------------------------------------------------------------------------------------
+// A workgroup takes 64 input channels; its eight wavefronts deal the output channels among themselves, 64 at a time, and join their sums in LDS.  A lane reads
+// eight rows of four codes and makes the operands of the four column tiles of them.  Each 64 numbers of a row have a power of two of their own, so nothing has to
+// be known of a row before the weight's first bytes are asked for.  Where that makes few workgroups for many output channels, the output channels are cut into runs
+// of `run` as well, and k8_dx_join adds the runs' results.
+template <class T, int NP>
+__global__ __launch_bounds__(512) void k8_dx_few(dn_i8_grad_desc d, int run, float *part) {
+    __shared__ __align__(16) float sums[8][4][256];
+    const int lane = threadIdx.x & 63, wave = k8_uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4, n = (int)d.n, m = (int)d.m;
+    const int64_t k0 = (int64_t)blockIdx.x * 64;
+    const int cols = (int)min((int64_t)64, d.k - k0);
+    const int64_t row = min(c, m - 1);                     // operand rows behind the last one repeat it
+    K8Raw<T, 8> x[2]; K8Raw<float, 8> sw[2]; unsigned bits[2], rows[2][8];
+    const T *px = (const T *)d.dy + row * d.ldy + 8 * g;
+    const uint8_t *pm = d.mask ? d.mask + row * d.ldmask : nullptr;
+    // four columns that end behind the matrix are read in front of its end and moved down
+    const int64_t at_k = min(k0 + 4 * c, d.k - 4);
+    const int down8 = 8 * (int)min(k0 + 4 * c - at_k, (int64_t)3);
+    const unsigned ldw = (unsigned)d.ldw, pw0 = (unsigned)(8 * g) * ldw + (unsigned)at_k;
+    typedef const __attribute__((address_space(1))) k8_u32 *gu32;
+    auto fetch = [&](int step, auto kind) __attribute__((always_inline)) {     // WHOLE: the row does not end here
+        constexpr bool WHOLE = decltype(kind)::value;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int at0 = step * 64 + s * 32, at = at0 + 8 * g;
+            if (WHOLE) { x[s].load(px + at0); sw[s].load(d.sw + at); }
+            else { x[s].load(px + at0, n - at); sw[s].load(d.sw + at, n - at); }
+            if (pm) bits[s] = pm[min(at, n - 1) >> 3];
+            const k8_global w = k8_base(d.w + at0 * d.ldw);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (WHOLE) rows[s][e] = *(gu32)(w + e * (int64_t)ldw + pw0);
+                else rows[s][e] = *(gu32)(k8_base(d.w) + (int64_t)min(at + e, n - 1) * ldw + at_k);            // zeros times the last row behind the end
+        }
+    };
+    k8_f32x4 sum[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) sum[t] = k8_f32x4{ 0, 0, 0, 0 };
+    const int steps = (min(n, ((int)blockIdx.y + 1) * run) + 63) / 64;         // (a run is whole steps)
+    auto next = [&](int step) __attribute__((always_inline)) {
+        if (step < steps && step * 64 + 64 <= n) fetch(step, std::true_type());
+        else if (step < steps) fetch(step, std::false_type());
+    };
+    const int first = (int)blockIdx.y * (run / 64) + wave;
+    next(first);
+    for (int step = first; step < steps; step += 8) {
+        float v[2][8], most = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                float z = x[s].get(e);
+                if (pm) z = __uint_as_float(__float_as_uint(z) & (unsigned)((int)(bits[s] << (31 - e)) >> 31));
+                v[s][e] = z * sw[s].get(e);
+                most = fmaxf(most, fabsf(v[s][e]));
+            }
+        if (__any(!(most <= 0x1.fffffep127f))) {           // the largest finite one
+            most = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) { const float a = fabsf(v[s][e]); most = fmaxf(most, a <= 0x1.fffffep127f ? a : 0.0f); }
+        }
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        const K8Pow pw = k8_pow(__float_as_uint(most));
+        i32x4 a[2][NP], b[2][4];
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+#pragma unroll
+            for (int p = 0; p < 4; p++) {
+                const float v0 = v[s][2 * p] * pw.up, v1 = v[s][2 * p + 1] * pw.up;
+                if (NP == 2) { const K8Split w = k8_split(v0, v1); a[s][0][p] = w.hi; a[s][NP - 1][p] = w.lo; }
+                else a[s][0][p] = k8_pack(v0, v1);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) rows[s][e] >>= down8;
+            k8_columns(rows[s], b[s]);
+        }
+        next(step + 8);
+        float down[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) down[i] = __shfl(pw.down, 4 * g + i);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            k8_f32x4 acc = { 0, 0, 0, 0 };
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int p = 0; p < NP; p++) acc = k8_mfma16(a[s][p], b[s][t], acc);
+#pragma unroll
+            for (int i = 0; i < 4; i++) sum[t][i] = __builtin_fmaf(acc[i], down[i], sum[t][i]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++)                            // D: column lane & 15, row 4 g + i
+#pragma unroll
+        for (int i = 0; i < 4; i++) sums[wave][t][(4 * g + i) * 16 + c] = sum[t][i];
+    __syncthreads();
+    const int kk = threadIdx.x & 63;
+    for (int r = threadIdx.x >> 6; r < m; r += 8) {
+        float v = 0.0f;
+#pragma unroll
+        for (int z = 0; z < 8; z++) v += sums[z][kk & 3][r * 16 + (kk >> 2)];
+        if (kk >= cols) continue;
+        if (part) part[((int64_t)blockIdx.y * m + r) * d.k + k0 + kk] = v;
+        else ((T *)d.dx)[r * d.ldx + k0 + kk] = (T)v;
     }
 }
 
@@ -376,6 +508,12 @@ __device__ __forceinline__ void k8_put4(void *p, int type, int64_t at, const flo
     if (type == DN_T_F32) k8_put4((float *)p + at, v, left);
     else if (type == DN_T_F16) k8_put4((_Float16 *)p + at, v, left);
     else k8_put4((k8_bf16 *)p + at, v, left);
+}
+
+__device__ __forceinline__ void k8_store_b(const dn_i8_grad_desc &d, int64_t n, float v) {
+    if (d.dw_type == DN_T_F32) ((float *)d.db)[n] = v;
+    else if (d.dw_type == DN_T_F16) ((_Float16 *)d.db)[n] = (_Float16)v;
+    else ((k8_bf16 *)d.db)[n] = (k8_bf16)v;
 }
 
 template <class T, int S, int NP>
@@ -425,7 +563,7 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const k8_global p = pu + up(e) * d.ldy * (int64_t)sizeof(T) + (row(e) * (unsigned)d.ldy + (unsigned)ch) * (unsigned)sizeof(T);
-                if (WHOLE || ch + 4 <= ncols) raw[e].load(p);
+                if (WHOLE || ncols == S) raw[e].load(p);
                 else raw[e].load(p, ncols - ch);
             }
             if (d.mask) {
@@ -444,11 +582,11 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const k8_global p = pq + up(e) * d.ldq + (row(e) * (unsigned)d.ldq + (unsigned)ch);
-                if (WHOLE || ch + 4 <= kcols) rq[e] = *(const __attribute__((address_space(1))) k8_u32 *)p;
-                else {
+                if (WHOLE || kcols == S) rq[e] = *(const __attribute__((address_space(1))) k8_u32 *)p;
+                else {                                     // (channels behind the last one repeat it; they are not stored)
                     rq[e] = 0u;
 #pragma unroll
-                    for (int j = 0; j < 3; j++) if (ch + j < kcols) rq[e] |= (unsigned)((gu8)p)[j] << (8 * j);
+                    for (int j = 0; j < 4; j++) rq[e] |= (unsigned)((gu8)p)[min(j, kcols - 1 - ch)] << (8 * j);
                 }
             }
         }
@@ -521,6 +659,30 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
         }
     };
     int stage = 0;
+    // the channels' powers from the tile in hand (its mask bits already shifted down if `down`), lowered where it does not fit; pw, power and lower are set
+    auto lower_powers = [&](int down) __attribute__((always_inline)) {
+        for (int i = tid; i < S; i += 512) peak[i] = 0u;
+        __syncthreads();
+        if (u_in)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                unsigned top = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) { const unsigned v = k8_mag((rbit[e] >> (down + j) & 1 ? raw[e].get(j) : 0.0f) * rs[e]); top = max(top, v < 0x7f800000u ? v : 0u); }
+                atomicMax(&peak[ch + j], top);
+            }
+        __syncthreads();
+        for (int i = tid; i < S; i += 512) {
+            const float was = power[i], a = __uint_as_float(peak[i]);
+            float now = was;
+            if (a * was > 32768.0f) now = __uint_as_float((unsigned)min(max(264 - (int)(peak[i] >> 23), 1), 253) << 23);     // a -> [2^10, 2^11)
+            power[i] = now;
+            lower[i] = now / was;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; j++) pw[j] = power[ch + j];
+    };
     // again, next: fetch this tile / the next one
     auto tile = [&](auto whole, auto &&again, auto &&next) __attribute__((always_inline)) {
         char *l = lds[stage];
@@ -535,28 +697,8 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
             __syncthreads();
             if (raised[stage]) {
                 again();
-                for (int i = tid; i < S; i += 512) peak[i] = 0u;
-                __syncthreads();
-                if (has_u)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        unsigned top = 0;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) { const unsigned v = k8_mag((rbit[e] >> (esh + j) & 1 ? raw[e].get(j) : 0.0f) * rs[e]); top = max(top, v < 0x7f800000u ? v : 0u); }
-                        atomicMax(&peak[ch + j], top);
-                    }
-                __syncthreads();
-                for (int i = tid; i < S; i += 512) {
-                    const float was = power[i], a = __uint_as_float(peak[i]);
-                    float now = was;
-                    if (a * was > 32768.0f) now = __uint_as_float((unsigned)min(max(264 - (int)(peak[i] >> 23), 1), 253) << 23);     // a -> [2^10, 2^11)
-                    power[i] = now;
-                    lower[i] = now / was;
-                }
+                lower_powers(esh);
                 if (tid == 0) raised[stage] = 0;
-                __syncthreads();
-#pragma unroll
-                for (int j = 0; j < 4; j++) pw[j] = power[ch + j];
 #pragma unroll
                 for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -578,11 +720,15 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
     // (a call without rows has one empty run: its sums are zeros)
     int64_t base = r0;
     const int64_t whole = min(r1, d.ldy && d.ldq ? d.m - 3 : (int64_t)0) - D::RT;         // the last tile that can be fetched whole starts here or before
-    if (base <= whole) fetch(base, std::true_type());
+    if (base <= whole) {
+        fetch(base, std::true_type());
+        if (with_q) lower_powers(esh);
+    }
     for (; base <= whole; base += D::RT) tile(std::true_type(), [&]() __attribute__((always_inline)) { fetch(base, std::true_type()); },
                                                         [&]() __attribute__((always_inline)) { if (base + D::RT <= whole) fetch(base + D::RT, std::true_type()); });
     for (; base < r1; base += D::RT) {
         fetch(base, std::false_type());
+        if (with_q && base == r0) lower_powers(esh);
         tile(std::false_type(), [&]() __attribute__((always_inline)) { fetch(base, std::false_type()); }, []() {});
     }
     // ---- the sums leave: sets of wavefronts joined in LDS first, in the order of the sets
@@ -635,11 +781,117 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
             float v = 0.0f;
             for (int r = 0; r < D::RT / 8; r++) v += js[r * S + i];
             if (!last) o.part_b[(int64_t)z * d.n + n0 + i] = v;
-            else if (d.dw_type == DN_T_F32) ((float *)d.db)[n0 + i] = v;
-            else if (d.dw_type == DN_T_F16) ((_Float16 *)d.db)[n0 + i] = (_Float16)v;
-            else ((k8_bf16 *)d.db)[n0 + i] = (k8_bf16)v;
+            else k8_store_b(d, n0 + i, v);
         }
     }
+}
+// ---- dw and db, few rows (M <= 16) ------------------------------------------------------------------------------------------------------------------------------
+// dw's bytes are all there is to move.  The factors dz s and the codes go as they are, in fp32, into matrix instructions over four rows; 64 x 64 results per wavefront,
+// tile t of a block holds input channels 4 c + t, so that a lane stores four adjacent ones.  No LDS, no waiting for one another.
+template <class T, class W>
+__global__ __launch_bounds__(256) void k8_dw_few(dn_i8_grad_desc d) {
+    const int lane = threadIdx.x & 63, wave = k8_uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4, m = (int)d.m;
+    const int64_t n0 = (int64_t)blockIdx.y * 64, k0 = (int64_t)blockIdx.x * 256 + wave * 64, left = d.k - k0 - 4 * c;
+    const bool with_q = d.dw && k0 < d.k;
+    float u[4][4], sum[4] = { 0, 0, 0, 0 }, scale[4] = { 0, 0, 0, 0 };
+    unsigned q[4] = { 0, 0, 0, 0 };
+    int64_t row[4], col[4];                                // rows 4 s + g; those behind the last one repeat it and count as zeros
+#pragma unroll
+    for (int s = 0; s < 4; s++) { row[s] = min(4 * s + g, m - 1); col[s] = min(n0 + 16 * s + c, d.n - 1); }
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) u[b][s] = (float)((const T *)d.dy)[row[s] * d.ldy + col[b]];
+    if (with_q) {
+#pragma unroll
+        for (int s = 0; s < 4; s++) scale[s] = d.s[row[s]];
+        const int8_t *p = d.q + k0 + 4 * c;
+        if (k0 + 64 <= d.k)
+#pragma unroll
+            for (int s = 0; s < 4; s++) __builtin_memcpy(&q[s], p + row[s] * d.ldq, 4);
+        else
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) q[s] |= (unsigned)(uint8_t)p[row[s] * d.ldq + min((int64_t)j, left - 1)] << (8 * j);        // the row's last code stands for those behind it
+    }
+    if (d.mask) {
+        unsigned bits[4][4];
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+            for (int b = 0; b < 4; b++) bits[b][s] = d.mask[row[s] * d.ldmask + (col[b] >> 3)];
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+            for (int b = 0; b < 4; b++) u[b][s] = bits[b][s] >> (col[b] & 7) & 1 ? u[b][s] : 0.0f;
+    }
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const float z = 4 * s + g < m ? u[b][s] : 0.0f;
+            sum[b] += z;
+            u[b][s] = 4 * s + g < m ? z * scale[s] : 0.0f;
+        }
+    if (with_q)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            k8_f32x4 acc[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                acc[t] = k8_f32x4{ 0, 0, 0, 0 };
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+                    if (4 * s < m) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(u[b][s], (float)(int8_t)(q[s] >> (8 * t)), acc[t], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int64_t n = n0 + 16 * b + 4 * g + i;
+                const float v[4] = { acc[0][i], acc[1][i], acc[2][i], acc[3][i] };
+                if (n < d.n && left > 0) k8_put4((W *)d.dw + n * d.lddw + k0 + 4 * c, v, left);
+            }
+        }
+    if (d.db && blockIdx.x == 0 && wave == 0)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            sum[b] += __shfl_xor(sum[b], 16);
+            sum[b] += __shfl_xor(sum[b], 32);
+            const int64_t n = n0 + 16 * b + c;
+            if (g == 0 && n < d.n) k8_store_b(d, n, sum[b]);
+        }
+}
+
+// few runs joined: a lane takes four adjacent results of all of them
+__global__ __launch_bounds__(256) void k8_dw_join_few(const float *__restrict__ part, const float *__restrict__ part_b, int splits, int64_t n, int64_t k, void *__restrict__ dw,
+                                                      int64_t lddw, void *__restrict__ db, int type, unsigned dw_blocks) {
+    const bool is_b = blockIdx.x >= dw_blocks;
+    const int64_t count = is_b ? n : n * k, at = ((int64_t)(is_b ? blockIdx.x - dw_blocks : blockIdx.x) * 256 + threadIdx.x) * 4, left = count - at;
+    if (left <= 0) return;
+    const float *p = (is_b ? part_b : part) + at;
+    float v[4] = { 0, 0, 0, 0 };
+    if (left >= 4)
+#pragma unroll 8
+        for (int z = 0; z < splits; z++) {
+            const K8Vec<float, 4> t = k8_load<float, 4>(p + (int64_t)z * count);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] += t.v[j];
+        }
+    else
+        for (int z = 0; z < splits; z++)
+#pragma unroll
+            for (int j = 0; j < 3; j++) if (j < left) v[j] += p[(int64_t)z * count + j];
+    void *out = is_b ? db : dw;
+    const int64_t r = is_b ? 0 : at / k, c = is_b ? at : at - r * k;
+    if (left >= 4 && (is_b || c + 4 <= k)) { k8_put4(out, type, is_b ? at : r * lddw + c, v, 4); return; }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (j < left) {
+            const int64_t o = is_b ? at + j : (at + j) / k * lddw + (at + j) % k;
+            if (type == DN_T_F32) ((float *)out)[o] = v[j];
+            else if (type == DN_T_F16) ((_Float16 *)out)[o] = (_Float16)v[j];
+            else ((k8_bf16 *)out)[o] = (k8_bf16)v[j];
+        }
 }
 // the runs joined, dw's and db's in one launch.  A workgroup takes 256 adjacent results: 64 lanes x four, 16 wavefronts a sixteenth of the runs each, so that a
 // run's loads are all in flight at once
@@ -685,7 +937,7 @@ __global__ __launch_bounds__(1024) void k8_dw_join(const float *__restrict__ par
 
 // ---- which way a call takes.  Nothing here looks at which results are asked for: a result's bits do not depend on its company -----------------------------------------
 struct Plan {
-    bool narrow = false, big = false; int dx_splits = 1, np_x = 1, np_w = 1, pitch = 0;
+    bool few = false, narrow = false, big = false; int dx_splits = 1, np_x = 1, np_w = 1, pitch = 0;
     int s = 256, tiles_n = 1, tiles_k = 1, splits = 1; int64_t run = 0;
     uint64_t pieces = 0, turned = 0, down = 0, dx_part = 0, part = 0, part_b = 0, total = 0;
 };
@@ -694,24 +946,45 @@ Plan plan_grad(const dn_i8_grad_desc &d) {
     auto take = [&](uint64_t bytes) { const uint64_t at = p.total; p.total += k8_up(bytes, 256); return at; };
     p.np_x = d.dy_type == DN_T_F32 ? 2 : 1;
     p.np_w = d.dw_type == DN_T_F32 ? 2 : 1;
-    p.narrow = d.n <= 256 && d.k <= 512;
+    p.few = d.m >= 1 && d.m <= 16 && d.k >= 4;
+    p.narrow = d.n <= 256 && d.k <= 1024;
+    if (p.few) {
+        p.dx_splits = (int)std::max<int64_t>(1, std::min<int64_t>(K8_CUS / ((d.k + 63) / 64), d.n / 1024));
+        if (d.dx && p.dx_splits > 1) p.dx_part = take((uint64_t)p.dx_splits * d.m * d.k * 4);
+        return p;
+    }
     if (d.dx && d.m && !p.narrow) {
         p.pitch = (int)k8_up(d.n, 8);
         p.pieces = take((uint64_t)p.np_x * d.m * p.pitch * 2);
         p.turned = take((uint64_t)d.k * p.pitch * 2);
         p.down = take((uint64_t)d.m * 4);
         const int64_t t256 = ((d.m + 255) / 256) * ((d.k + 255) / 256), t128 = ((d.m + 127) / 128) * ((d.k + 127) / 128), steps = (p.pitch * 2 + 127) / 128 * p.np_x;
-        p.big = t256 >= K8_CUS;
+        p.big = t256 >= K8_CUS && d.k > 64;
         if (!p.big && t128 < K8_CUS) {
             p.dx_splits = (int)std::max<int64_t>(1, std::min<int64_t>(K8_CUS / t128, steps / 4));
             if (p.dx_splits > 1) p.dx_part = take((uint64_t)p.dx_splits * d.m * d.k * 4);
         }
     }
-    const int64_t widest = std::max(d.n, d.k);
-    p.s = widest <= 64 ? 64 : widest <= 128 ? 128 : 256;
+    int64_t want = K8_CUS;
+    // dw's tiles and the runs of rows: what costs least, by times measured on whole chips -- a workgroup's row in a tile of 256: 55 ns, of 128: 21; its start and end:
+    // 14 us and 9; a run's results, written and read again: 1.2 ps each.  bf16, us, 256 : 128 -- 1048576 x 256 x 256, 281 : 345; 200000 x 192 x 192, 73 : 89;
+    // 50000 x 1024 x 256, 103 : 85; 7552 x 1664 x 1216, 82 : 139; 1000 x 1024 x 1024, 39 : 23; 64 x 2048 x 4096, 20 : 26
+    if (std::max(d.n, d.k) <= 64) p.s = 64;
+    else {
+        double least = 1e30;
+        for (int side : { 128, 256 }) {
+            const int64_t tiles = ((d.n + side - 1) / side) * ((d.k + side - 1) / side), most = std::max<int64_t>(1, (d.m * p.np_w * side + 16383) / 16384);
+            for (int rounds = 1; rounds <= 3; rounds++) {
+                const int64_t runs = std::min(most, std::max<int64_t>(1, rounds * K8_CUS / tiles)), turns = (tiles * runs + K8_CUS - 1) / K8_CUS;
+                const double cost = (double)turns * ((side == 256 ? 14e3 : 9e3) + (side == 256 ? 55.0 : 21.0) * (double)(d.m * p.np_w) / (double)runs) +
+                                    (runs > 1 ? 3e3 + 1.2e-3 * (double)(runs * d.n * d.k) : 0.0);
+                if (cost < least) { least = cost; p.s = side; want = runs; }
+            }
+        }
+    }
     const int64_t rt = 16384 / p.s / p.np_w, row_tiles = std::max<int64_t>(1, (d.m + rt - 1) / rt);
     p.tiles_n = (int)((d.n + p.s - 1) / p.s); p.tiles_k = (int)((d.k + p.s - 1) / p.s);
-    const int64_t want = std::max<int64_t>(1, K8_CUS / ((int64_t)p.tiles_n * p.tiles_k)), each = (row_tiles + want - 1) / want;
+    const int64_t each = (row_tiles + want - 1) / want;
     p.run = each * rt;
     p.splits = (int)((row_tiles + each - 1) / each);
     if (p.splits > 1) {
@@ -722,16 +995,24 @@ Plan plan_grad(const dn_i8_grad_desc &d) {
 }
 
 template <class T, int NP, class Epi> hipError_t dx_gemm(const dn_i8_grad_desc &d, const Plan &p, char *base, const Epi &e, hipStream_t st) {
-    const int b = p.big ? 256 : 128;
+    const int b = p.big ? 256 : 128, bk = p.big || d.k > 64 ? b : 64;
     const int64_t plane = d.m * (int64_t)p.pitch * 2;
     G8 g = { base + p.pieces, base + p.turned, (int64_t)p.pitch * 2, (int64_t)p.pitch * 2, d.m, d.k, p.pitch * 2, NP, plane, p.dx_splits,
-             (int)((d.m + b - 1) / b), (int)((d.k + b - 1) / b) };
+             (int)((d.m + b - 1) / b), (int)((d.k + bk - 1) / bk) };
     const unsigned grid = (unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits);
-    if (p.big) k8_gemm<false, 256, 256, 2, 4, Epi><<<dim3(grid), 512, 0, st>>>(g, e);
+    if (bk == 64) k8_gemm<false, 128, 64, 4, 1, Epi><<<dim3(grid), 256, 0, st>>>(g, e);
+    else if (p.big) k8_gemm<false, 256, 256, 2, 4, Epi><<<dim3(grid), 512, 0, st>>>(g, e);
     else k8_gemm<false, 128, 128, 2, 2, Epi><<<dim3(grid), 256, 0, st>>>(g, e);
     return hipGetLastError();
 }
 template <class T, int NP> hipError_t dx_of(const dn_i8_grad_desc &d, const Plan &p, char *base, hipStream_t st) {
+    if (p.few) {
+        const int run = (int)k8_up((d.n + p.dx_splits - 1) / p.dx_splits, 64);
+        float *part = p.dx_splits > 1 ? (float *)(base + p.dx_part) : nullptr;
+        k8_dx_few<T, NP><<<dim3((unsigned)((d.k + 63) / 64), (unsigned)p.dx_splits), 512, 0, st>>>(d, run, part);
+        if (part) k8_dx_join<T><<<dim3((unsigned)((d.m * ((d.k + 255) / 256) + 3) / 4)), 256, 0, st>>>(part, p.dx_splits, nullptr, (T *)d.dx, d.m, d.k, d.ldx);
+        return hipGetLastError();
+    }
     if (p.narrow) {
         const unsigned per = (unsigned)((d.k + 255) / 256);
         auto grid = [&](int wg, int each) { return dim3((unsigned)std::min<int64_t>((d.m + wg / 4 - 1) / (wg / 4), each * K8_CUS / per), per); };      // a wavefront has 16 rows
@@ -757,6 +1038,13 @@ template <class T, int NP> hipError_t dx_of(const dn_i8_grad_desc &d, const Plan
     return hipGetLastError();
 }
 template <class T, int NP> hipError_t dw_of(const dn_i8_grad_desc &d, const Plan &p, char *base, hipStream_t st) {
+    if (p.few) {
+        const dim3 grid(d.dw ? (unsigned)((d.k + 255) / 256) : 1u, (unsigned)((d.n + 63) / 64));
+        if (d.dw_type == DN_T_F32) k8_dw_few<T, float><<<grid, 256, 0, st>>>(d);
+        else if (d.dw_type == DN_T_F16) k8_dw_few<T, _Float16><<<grid, 256, 0, st>>>(d);
+        else k8_dw_few<T, k8_bf16><<<grid, 256, 0, st>>>(d);
+        return hipGetLastError();
+    }
     const int tiles_k = d.dw ? p.tiles_k : 1;
     const DwOut o = { (float *)(base + p.part), (float *)(base + p.part_b), p.splits, p.tiles_n, tiles_k, p.run };
     const dim3 grid((unsigned)((int64_t)p.splits * p.tiles_n * tiles_k));
@@ -764,8 +1052,10 @@ template <class T, int NP> hipError_t dw_of(const dn_i8_grad_desc &d, const Plan
     else if (p.s == 128) k8_dw<T, 128, NP><<<grid, 512, 0, st>>>(d, o);
     else k8_dw<T, 256, NP><<<grid, 512, 0, st>>>(d, o);
     if (p.splits > 1) {
-        const unsigned dw_blocks = d.dw ? (unsigned)((d.n * d.k + 255) / 256) : 0, db_blocks = d.db ? (unsigned)((d.n + 255) / 256) : 0;
-        k8_dw_join<<<dim3(dw_blocks + db_blocks), 1024, 0, st>>>(o.part, o.part_b, p.splits, d.n, d.k, d.dw, d.lddw, d.db, d.dw_type, dw_blocks);
+        const int64_t each = p.splits > 32 && d.n * d.k < 1024 * K8_CUS ? 256 : 1024;
+        const unsigned dw_blocks = d.dw ? (unsigned)((d.n * d.k + each - 1) / each) : 0, db_blocks = d.db ? (unsigned)((d.n + each - 1) / each) : 0;
+        if (each == 1024) k8_dw_join_few<<<dim3(dw_blocks + db_blocks), 256, 0, st>>>(o.part, o.part_b, p.splits, d.n, d.k, d.dw, d.lddw, d.db, d.dw_type, dw_blocks);
+        else k8_dw_join<<<dim3(dw_blocks + db_blocks), 1024, 0, st>>>(o.part, o.part_b, p.splits, d.n, d.k, d.dw, d.lddw, d.db, d.dw_type, dw_blocks);
     }
     return hipGetLastError();
 }
