@@ -198,3 +198,92 @@ def linear_grad(ctx, dy, q, s, wq, ws, mask=None, need_dx=True, need_dw=True, ne
         _run(ctx, "dn_i8_linear_grad", hip.I8_GRAD.pack(m, n, k, dy.data_ptr(), ldy, at_mask, ldmask, q.data_ptr(), ldq, at_s, wq.data_ptr(), ldw, at_ws,
                                                         at_dx, k, at_dw, k, at_db, TYPES[dy.dtype], TYPES[w_dtype]))
     return dx, dw, db
+
+
+# ---- the layer that is trained with them ----------------------------------------------------------------------------------------------------------------
+def _packed(t):
+    """t, or a copy without gaps if its rows do not lie at one pitch (the gradient of a sum is one number repeated, for instance)"""
+    try:
+        _rows("", t)
+        return t
+    except ValueError:
+        return t.contiguous()
+
+
+class _Layer(torch.autograd.Function):
+    """The forward pass keeps what i8_linear saves and the weight's 8-bit rows; both quantisers count as the identity in the backward pass, so the gradients
+    are those of the product that was computed."""
+
+    @staticmethod
+    def forward(fn, x, weight, bias, residual, ctx, relu):
+        wq, ws = rows(ctx, _packed(weight))
+        b = None if bias is None else bias.float()
+        y, saved = linear(ctx, _packed(x), wq, ws, bias=b, residual=None if residual is None else _packed(residual), relu=relu, save=True)
+        fn.save_for_backward(saved.q, saved.s, saved.mask, wq, ws)
+        fn.ctx, fn.w_dtype, fn.b_dtype = ctx, weight.dtype, None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(fn, dy):
+        q, s, mask, wq, ws = fn.saved_tensors
+        need_x, need_w, need_b, need_r = fn.needs_input_grad[:4]
+        dr = None
+        if need_r:
+            dr = dy
+            if mask is not None:
+                bits = torch.arange(dy.shape[-1], device=dy.device)
+                keep = mask[:, bits >> 3].bitwise_right_shift((bits & 7).to(_U8)).bitwise_and(1).bool()
+                dr = torch.where(keep.view(dy.shape), dy, torch.zeros((), dtype=dy.dtype, device=dy.device))
+        dx, dw, db = linear_grad(fn.ctx, _packed(dy), q, s, wq, ws, mask, need_x, need_w, need_b, fn.w_dtype)
+        return dx, dw, db if db is None else db.to(fn.b_dtype), dr, None, None
+
+
+class Dense(torch.nn.Module):
+    """y [..., N] = act(x W^T + b (+ residual)) whose forward pass multiplies 8-bit rows and whose backward pass reads them again: weight [N, K] and bias [N] are
+    parameters (fp32, fp16 or bf16) on ctx's device; x [..., K] of the same types.  Between the passes a row of x costs K + 4 bytes.
+
+    A pass can be captured into a graph like any of torch's (its workspaces are torch tensors); as with those, no eager graph over the same parameters
+    may be alive while a backward pass is being captured.
+
+    A pointwise convolution of a model description (cnn_model.py: an op "conv" with k = 1) is such a layer over positions: from_op() reads it, store() writes it
+    back, so that a description can be fitted here and run by Context.load_cnn."""
+
+    def __init__(self, ctx, k, n, bias=True, relu=False, dtype=torch.float32):
+        super().__init__()
+        if dtype not in _NUMBERS:
+            raise TypeError("dtype is %s" % dtype)
+        device = torch.device("cuda", ctx.device)
+        self.ctx, self.relu = ctx, bool(relu)
+        self.weight = torch.nn.Parameter((torch.randn(n, k, device=device) * k ** -0.5).to(dtype))
+        self.bias = torch.nn.Parameter(torch.zeros(n, dtype=dtype, device=device)) if bias else None
+
+    def forward(self, x, residual=None):
+        return _Layer.apply(x, self.weight, self.bias, residual, self.ctx, self.relu)
+
+    @staticmethod
+    def _op(desc, i):
+        op = desc["ops"][i]
+        if op["op"] != "conv" or op["k"] != 1:
+            raise ValueError("op %d is no pointwise convolution" % i)
+        return op, op["cin"], op["cout"]
+
+    @classmethod
+    def from_op(cls, ctx, desc, blob, i, dtype=torch.float32):
+        """op i of a description: W = kernel^T times the folded BatchNorm's factor, b = its shift.  An op that adds a buffer (add >= 0) takes it as `residual`."""
+        op, k, n = cls._op(desc, i)
+        w = torch.from_numpy(blob[op["w"]:op["w"] + k * n].reshape(k, n).copy()).t() * torch.from_numpy(blob[op["scale"]:op["scale"] + n].copy())[:, None]
+        layer = cls(ctx, k, n, relu=op["relu"], dtype=dtype)
+        with torch.no_grad():
+            layer.weight.copy_(w)
+            layer.bias.copy_(torch.from_numpy(blob[op["shift"]:op["shift"] + n].copy()))
+        return layer
+
+    def store(self, desc, blob, i):
+        """the parameters into op i of the description's blob, in place: the kernel holds W^T, the factor becomes one"""
+        op, k, n = self._op(desc, i)
+        if (n, k) != tuple(self.weight.shape) or op["relu"] != self.relu:
+            raise ValueError("op %d has another shape or activation than this layer" % i)
+        blob[op["w"]:op["w"] + k * n] = self.weight.detach().float().t().reshape(-1).cpu().numpy()
+        blob[op["scale"]:op["scale"] + n] = 1.0
+        blob[op["shift"]:op["shift"] + n] = 0.0 if self.bias is None else self.bias.detach().float().cpu().numpy()

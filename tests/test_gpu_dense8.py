@@ -490,3 +490,244 @@ def test_refusals(ctx):
                        (lambda: ctx.i8_linear_grad(dy.sum().expand(6, 8), q, s, wq, ws), ValueError), (lambda: ctx.i8_linear_grad(dy, q, s, wq, ws, w_dtype=torch.float64), TypeError)]:
         with pytest.raises(kind):
             call()
+
+
+# ---- shapes at which a call takes another way: few output channels, few rows, long and short runs ------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("m,n,k", [(300, 64, 300), (5000, 39, 700), (200, 1, 500), (65, 17, 5000), (129, 65, 300), (300, 300, 115)])
+def test_linear_of_few_channels_with_residual(ctx, m, n, k, dtype):
+    x = some_rows(m, k, dtype, m + n)
+    wq, ws = eight(n, k, m)
+    wide = torch.randn(m, n + 3, generator=gen(21), device="cuda").to(dtype)
+    want, t = linear_ref(*codes(x), wq, ws)
+    for res in (wide[:, 1:n + 1], wide[:1, :n].expand(m, n), wide[:, 3:].contiguous()):
+        y, saved = ctx.i8_linear(x, wq, ws, residual=res, relu=True, save=True)
+        r = res.double().cpu()
+        within(y, (want + r).clamp(min=0), t + r.abs(), dtype, 6 * 2.0 ** -24)
+        on = bits(saved.mask, n)
+        assert on[y.cpu() > 0].all() and not on[want + r < -8 * 2.0 ** -24 * (t + r.abs())].any()
+
+
+@pytest.mark.parametrize("dtype,w_dtype,relu", [(F32, F32, True), (F16, F16, False), (BF16, F32, True), (F32, F16, False)])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 4), (16, 1, 3), (7, 2100, 70), (16, 5000, 130), (3, 2049, 4), (12, 300, 1000), (16, 64, 64), (2, 1, 4100), (9, 1024, 1),
+                                   (17, 65, 66), (500, 40, 1024), (40, 256, 1000), (300, 600, 64), (300, 600, 33), (20000, 300, 130), (3000, 640, 200)])
+def test_grad_of_few_rows_and_few_channels(ctx, m, n, k, dtype, w_dtype, relu):
+    case = grad_case(m, n, k, dtype, m + n + k, relu)
+    got = ctx.i8_linear_grad(*case[:5], mask=case[5], w_dtype=w_dtype)
+    check_grad(got, grad_ref(*case), m, n, dtype, w_dtype)
+    for need in ((True, False, False), (False, True, False), (False, False, True)):
+        part = ctx.i8_linear_grad(*case[:5], mask=case[5], w_dtype=w_dtype, need_dx=need[0], need_dw=need[1], need_db=need[2])
+        assert all((p is not None) == want and (p is None or torch.equal(p, full)) for want, p, full in zip(need, part, got))
+
+
+@pytest.mark.parametrize("n,k", [(70, 40), (2500, 67), (9, 3)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_grad_of_few_rows_that_are_not_finite(ctx, n, k, dtype):
+    dy, q, s, wq, ws, mask = grad_case(8, n, k, dtype, 17, True)
+    keep = bits(mask, n)
+    keep[2], keep[3], keep[5] = False, True, False
+    mask = torch.from_numpy(np.packbits(keep.numpy(), axis=1, bitorder="little")).cuda()
+    ref = grad_ref(dy, q, s, wq, ws, mask)
+    clean = ctx.i8_linear_grad(dy, q, s, wq, ws, mask=mask)
+    check_grad(clean, ref, 8, n, dtype, dtype)
+    dy = dy.clone()
+    dy[2], dy[5, ::2], dy[5, 1::2] = float("nan"), float("inf"), float("-inf")             # all masked
+    for a, b in zip(ctx.i8_linear_grad(dy, q, s, wq, ws, mask=mask), clean):
+        assert torch.equal(a, b)
+    dy[3, 7] = float("nan")                                # kept
+    dx, dw, db = ctx.i8_linear_grad(dy, q, s, wq, ws, mask=mask)
+    assert dx[3].isnan().all() and dw[7].isnan().all() and db[7].isnan()
+    rows_, cols = [r for r in range(8) if r != 3], [c for c in range(n) if c != 7]
+    assert torch.equal(dx[rows_], clean[0][rows_]) and torch.equal(dw[cols], clean[1][cols]) and torch.equal(db[cols], clean[2][cols])
+
+
+def test_grad_of_few_rows_reads_strided_tensors(ctx):
+    m, n, k = 11, 1100, 70
+    dy, q, s, wq, ws, mask = grad_case(m, n, k, BF16, 5, True)
+    ref = grad_ref(dy, q, s, wq, ws, mask)
+    wide = torch.zeros(m, n + 9, dtype=BF16, device="cuda")
+    wide[:, 3:3 + n] = dy
+    qo = torch.zeros(m * (k + 1) + 1, dtype=torch.int8, device="cuda")[1:].view(m, k + 1)[:, :k]
+    qo.copy_(q)
+    wo = torch.zeros(n * k + 5, dtype=torch.int8, device="cuda")[5:].view(n, k)             # its last row ends where its memory ends
+    wo.copy_(wq)
+    mw = torch.zeros(m, (n + 7) // 8 + 2, dtype=torch.uint8, device="cuda")
+    mw[:, 1:-1] = mask
+    check_grad(ctx.i8_linear_grad(wide[:, 3:3 + n], qo, s, wo, ws, mask=mw[:, 1:-1]), ref, m, n, BF16, BF16)
+    one = ctx.i8_linear_grad(dy[:1].expand(m, n), q, s, wq, ws)
+    check_grad(one, grad_ref(dy[:1].expand(m, n), q, s, wq, ws, None), m, n, BF16, BF16)
+
+
+# ---- the layer that is trained ------------------------------------------------------------------------------------------------------------------------------
+def plain_layer(layer, x, residual=None):
+    """the layer in 64 bits over the numbers that its 8-bit rows stand for, as leaves: (y, x, w, b, residual)"""
+    leaf = lambda t: t.detach().double().cpu().requires_grad_()  # noqa: E731
+    q, s = codes(x.reshape(-1, x.shape[-1]))
+    xh = leaf((torch.from_numpy(q).double() * torch.from_numpy(s).double()[:, None]).view(x.shape))
+    wq, ws = codes(layer.weight)
+    wh = leaf(torch.from_numpy(wq).double() * torch.from_numpy(ws).double()[:, None])
+    b = None if layer.bias is None else leaf(layer.bias)
+    r = None if residual is None else leaf(residual)
+    y = xh @ wh.t()
+    for t in (b, r):
+        y = y if t is None else y + t
+    return (y.clamp(min=0) if layer.relu else y), xh, wh, b, r
+
+
+@pytest.mark.parametrize("dtype,p_dtype,relu,bias", [(F32, F32, True, True), (BF16, F32, True, True), (F16, F16, False, True), (BF16, BF16, False, False)])
+@pytest.mark.parametrize("shape,n", [((3, 5, 40), 24), ((1, 64), 300), ((700, 256), 256), ((130, 520), 65), ((0, 40), 24)])
+def test_layer_gradients(ctx, shape, n, dtype, p_dtype, relu, bias):
+    from dnascent_amd import dense8
+    torch.manual_seed(5)
+    layer = dense8.Dense(ctx, shape[-1], n, bias=bias, relu=relu, dtype=p_dtype)
+    if bias:
+        with torch.no_grad():
+            layer.bias.normal_()
+    m = math.prod(shape[:-1])
+    x = torch.randn(shape, generator=gen(1), device="cuda").to(dtype).requires_grad_()
+    res = torch.randn(shape[:-1] + (n,), generator=gen(2), device="cuda").to(dtype).requires_grad_()
+    dy = torch.randn(shape[:-1] + (n,), generator=gen(3), device="cuda").to(dtype)
+    y = layer(x, res)
+    y.backward(dy)
+    want, xh, wh, b, r = plain_layer(layer, x, res)
+    live = (y.detach().cpu() > 0) if relu else torch.ones(y.shape, dtype=torch.bool)       # a sum within a rounding of zero may fall on either side
+    dz = torch.where(live, dy.cpu().double(), torch.zeros((), dtype=torch.float64)).view(m, n)
+    x2, w2 = xh.detach().view(m, shape[-1]), wh.detach()
+    mag = x2.abs() @ w2.abs().t() + (b.detach().abs() if bias else 0) + r.detach().abs().view(m, n)
+    within(y.detach().view(m, n), want.detach().view(m, n), mag, dtype, 6 * 2.0 ** -24)
+    ref = (dz @ w2, dz.t() @ x2, dz.sum(0)), (dz.abs() @ w2.abs(), dz.abs().t() @ x2.abs(), dz.abs().sum(0))
+    got = (x.grad.view(m, shape[-1]), layer.weight.grad, layer.bias.grad if bias else ref[0][2].to(p_dtype).cuda())
+    assert layer.weight.grad.dtype == p_dtype and x.grad.dtype == dtype
+    check_grad(got, ref, m, n, dtype, p_dtype)
+    assert torch.equal(res.grad.double().cpu().view(m, n), dz)
+    if not relu and m:                                     # and against differences of the plain layer: linear, so a step of any size will do
+        (want * dy.cpu().double()).sum().backward()
+        d = torch.randn(w2.shape, dtype=torch.float64)
+        up, down = ((x2 @ (w2 + f * d).t() * dz).sum() for f in (0.5, -0.5))
+        assert abs((wh.grad * d).sum() - (up - down)) <= 1e-9 * (ref[1][1] * d.abs()).sum()
+
+
+def test_layer_shared_broadcast_frozen_and_summed(ctx):
+    from dnascent_amd import dense8
+    torch.manual_seed(6)
+    layer = dense8.Dense(ctx, 48, 48, relu=False)
+    x = torch.randn(1, 48, device="cuda").requires_grad_()
+    layer(x.expand(20, 48)).sum().backward()               # one row read twenty times; the gradient of a sum is one number repeated
+    w, wx = layer.weight.grad.clone(), x.grad.clone()
+    y, xh, wh, b, _ = plain_layer(layer, x)
+    (20 * y.sum()).backward()
+    mag = 20 * wh.detach().abs().sum(0, keepdim=True)
+    within(wx, xh.grad, mag, F32, 2.0 ** -21 + 68 * 2.0 ** -24)
+    within(w, wh.grad, 20 * xh.detach().abs().expand(48, 48), F32, 2.0 ** -21 + 20 * 2.0 ** -24)
+    layer.zero_grad()
+    a = layer(x.detach())                                  # twice through one weight: its gradients add up
+    layer(a).backward(torch.ones(1, 48, device="cuda"))
+    first = [p.grad.clone() for p in layer.parameters()]
+    layer.zero_grad()
+    mid = a.detach().requires_grad_()
+    layer(mid).backward(torch.ones(1, 48, device="cuda"))
+    layer(x.detach()).backward(mid.grad)
+    assert all(torch.allclose(p.grad, f, rtol=2.0 ** -22, atol=1e-6) for p, f in zip(layer.parameters(), first))
+    layer.zero_grad()
+    layer.weight.requires_grad_(False)
+    layer(x).sum().backward()
+    assert layer.weight.grad is None and layer.bias.grad is not None
+    with torch.no_grad():
+        assert not layer(x).requires_grad
+    t = torch.randn(48, 30, device="cuda").t()             # elements of a row not next to each other
+    assert torch.equal(layer(t), layer(t.contiguous()))
+    y = layer(x)
+    g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)                    # no second derivatives
+
+
+def test_layer_run_and_captured(ctx):
+    """two layers one after the other, fitted for a few steps: eagerly, and the same steps as one captured graph that is replayed with eager work in between"""
+    from dnascent_amd import dense8
+
+    def fresh():
+        torch.manual_seed(7)
+        return torch.nn.ModuleList([dense8.Dense(ctx, 64, 256, relu=True), dense8.Dense(ctx, 256, 64)])
+    x = torch.randn(500, 64, generator=gen(1), device="cuda")
+    target = torch.randn(500, 64, generator=gen(2), device="cuda")
+
+    def step(net):
+        y = net[1](net[0](x), x)
+        grads = torch.autograd.grad(y, list(net.parameters()), (y.detach() - target) * (2.0 / 500))        # of the squared error's sum over channels, mean over rows
+        with torch.no_grad():
+            for p, g in zip(net.parameters(), grads):
+                p.sub_(g, alpha=0.01)
+        return y.detach()
+    eager, captured = fresh(), fresh()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        step(fresh())
+    torch.cuda.current_stream().wait_stream(st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(captured)
+    for rep in range(4):
+        want = step(eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), rep
+        assert all(torch.equal(a, b) for a, b in zip(eager.parameters(), captured.parameters())), rep
+
+
+def test_layer_of_a_description(ctx):
+    """a pointwise convolution leaves a description, is used and fitted as a layer, and goes back: the network runs with it"""
+    from dnascent_amd import cnn_model, dense8
+    desc, blob, _ = cnn_model.default_model(3)
+    i = next(j for j, op in enumerate(desc["ops"]) if op["op"] == "conv" and op["k"] == 1 and op["relu"])
+    op = desc["ops"][i]
+    layer = dense8.Dense.from_op(ctx, desc, blob, i)
+    assert layer.relu and tuple(layer.weight.shape) == (op["cout"], op["cin"])
+    lens = np.array([200, 90], np.uint32)
+    rng = np.random.default_rng(1)
+    inputs = lens, rng.integers(1, 1025, 290).astype(np.float32), rng.integers(1, 257, 290).astype(np.float32), rng.normal(0, 1, (290, 20)).astype(np.float32)
+
+    def probabilities(b):
+        c = hip.Context(0)
+        c.load_cnn(desc, b)
+        p = c.cnn_infer(*inputs)
+        c.close()
+        return p
+    same, moved = blob.copy(), blob.copy()
+    layer.store(desc, same, i)
+    k, n = op["cin"], op["cout"]
+    folded = blob[op["w"]:op["w"] + k * n].reshape(k, n) * blob[op["scale"]:op["scale"] + n]
+    assert np.array_equal(same[op["w"]:op["w"] + k * n].reshape(k, n), folded) and (same[op["scale"]:op["scale"] + n] == 1).all()
+    before = probabilities(blob)
+    assert np.abs(probabilities(same) - before).max() < 1e-4               # the factor is in the kernel now: roundings only
+    x = torch.randn(290, k, generator=gen(4), device="cuda")
+    layer(x).square().sum(-1).mean().backward()
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.sub_(p.grad, alpha=0.5)
+    layer.store(desc, moved, i)
+    assert np.array_equal(moved[op["w"]:op["w"] + k * n].reshape(k, n), layer.weight.detach().cpu().numpy().T)
+    after = probabilities(moved)
+    assert np.abs(after - before).max() > 1e-4 and np.allclose(after.sum(1), 1, atol=1e-5)
+    back = dense8.Dense.from_op(ctx, desc, moved, i)
+    assert torch.equal(back.weight, layer.weight) and torch.equal(back.bias, layer.bias)
+
+
+def test_layer_refusals(ctx):
+    from dnascent_amd import cnn_model, dense8
+    desc, blob, _ = cnn_model.default_model(3)
+    layer = dense8.Dense(ctx, 8, 4)
+    with pytest.raises(ValueError):
+        layer(torch.zeros(3, 9, device="cuda"))
+    with pytest.raises(ValueError):
+        layer(torch.zeros(3, 8))
+    with pytest.raises(ValueError):
+        layer(torch.zeros(3, 8, device="cuda", dtype=torch.int8))
+    with pytest.raises(TypeError):
+        dense8.Dense(ctx, 8, 4, dtype=torch.float64)
+    with pytest.raises(ValueError):
+        dense8.Dense.from_op(ctx, desc, blob, 0)
+    i = next(j for j, op in enumerate(desc["ops"]) if op["op"] == "conv" and op["k"] == 1)
+    with pytest.raises(ValueError):
+        layer.store(desc, blob, i)
