@@ -571,7 +571,7 @@ __global__ __launch_bounds__(512) void k8_narrow(const X *__restrict__ x, int64_
 // ---- which way a call takes ---------------------------------------------------------------------------------------------------------------------------------
 enum { FEW, NARROW, WIDE };
 struct Plan {
-    int way = WIDE, splits = 1; bool big = false, inside = false;
+    int way = WIDE, splits = 1; K8Tiling tile = K8_BIG; bool inside = false;
     uint64_t q = 0, s = 0, x = 0, w = 0, part = 0, total = 0;   // places in the workspace
     int64_t ldq = 0;
 };
@@ -592,24 +592,13 @@ Plan plan_linear(const dn_i8_linear_desc &d) {
     if (p.way == FEW) return p;
     if (given ? !k8_direct(d.x, d.ldx) : d.q && !k8_direct(d.q, d.ldq)) p.x = take((uint64_t)d.m * k8_up(d.k, 16));
     if (!k8_direct(d.w, d.ldw)) p.w = take((uint64_t)d.n * k8_up(d.k, 16));
-    const int64_t t256 = ((d.m + 255) / 256) * ((d.n + 255) / 256), t128 = ((d.m + 127) / 128) * ((d.n + 127) / 128), steps = (d.k + 127) / 128;
-    p.big = t256 >= K8_CUS && d.n > 64;
-    if (!p.big && t128 < K8_CUS) {                         // fewer tiles than compute units: the reduction is cut, four steps at least to a run
-        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(K8_CUS / t128, steps / 4));
+    p.tile = k8_tiling(d.m, d.n);
+    const int64_t tiles = k8_tiles(p.tile, d.m, d.n);
+    if (tiles < K8_CUS) {                                  // fewer tiles than compute units: the reduction is cut, four steps at least to a run
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(K8_CUS / tiles, ((d.k + 127) / 128) / 4));
         if (p.splits > 1) p.part = take((uint64_t)p.splits * d.m * d.n * 4);
     }
     return p;
-}
-
-template <class Epi> hipError_t gemm_i8(G8 g, bool big, const Epi &e, hipStream_t st) {
-    const bool slim = g.n <= 64;
-    const int bm = big ? 256 : 128, bn = big ? 256 : slim ? 64 : 128;
-    g.tiles_m = (int)((g.m + bm - 1) / bm); g.tiles_n = (int)((g.n + bn - 1) / bn);
-    const unsigned grid = (unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits);
-    if (slim) k8_gemm<true, 128, 64, 4, 1, Epi><<<dim3(grid), 256, 0, st>>>(g, e);
-    else if (big) k8_gemm<true, 256, 256, 2, 4, Epi><<<dim3(grid), 512, 0, st>>>(g, e);
-    else k8_gemm<true, 128, 128, 2, 2, Epi><<<dim3(grid), 256, 0, st>>>(g, e);
-    return hipGetLastError();
 }
 
 }  // namespace
@@ -677,11 +666,11 @@ hipError_t k8_linear(const dn_i8_linear_desc &d, void *ws, hipStream_t st) {
     G8 g = { (const char *)q, (const char *)w, ldq, ldw, d.m, d.n, (int)d.k, 1, 0, p.splits, 0, 0 };
     if (p.splits > 1) {
         const PartEpi e = { (int *)(base + p.part), d.m, d.n };
-        const hipError_t err = gemm_i8(g, p.big, e, st);
+        const hipError_t err = k8_product<true>(g, p.tile, e, st);
         if (err != hipSuccess) return err;
         const unsigned grid = (unsigned)((d.m * ((d.n + 255) / 256) + 3) / 4);
         K8_TYPE(d.y_type, T, k8_join<T><<<dim3(grid), 256, 0, st>>>(e.part, p.splits, o));
         return hipGetLastError();
     }
-    K8_TYPE(d.y_type, T, return gemm_i8(g, p.big, LinearEpi<T>{ o }, st));
+    K8_TYPE(d.y_type, T, return k8_product<true>(g, p.tile, LinearEpi<T>{ o }, st));
 }

@@ -181,3 +181,25 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k8_gemm(G8 g, Epi epi) {
         }
     }
 }
+
+// Which tiles a product takes: 256 x 256 where that makes a tile for every compute unit, 128 x 128 where that does, 128 x 64 otherwise and where b has no more rows.
+// us, the larger : the smaller tile -- 328813 x 1344 x 39 fp16, 402 (256) : 150 (64); 1500 x 2048 x 1605 bf16, 32 (128) : 25 (64); 500 x 500 x 500, 18 (128) : 12 (64);
+// 200 x 4096 x 2048 of a gradient, 19 (128) : 20 (64); with the operands of 8192 x 4096 x 4096 a tile of 256 reads half as much as one of 128
+enum K8Tiling { K8_BIG, K8_MIDDLE, K8_SLIM };
+inline int64_t k8_tiles(K8Tiling t, int64_t m, int64_t n) {
+    const int64_t bm = t == K8_BIG ? 256 : 128, bn = t == K8_BIG ? 256 : t == K8_MIDDLE ? 128 : 64;
+    return ((m + bm - 1) / bm) * ((n + bn - 1) / bn);
+}
+inline K8Tiling k8_tiling(int64_t m, int64_t n) {
+    if (n <= 64 || k8_tiles(K8_MIDDLE, m, n) < 256) return K8_SLIM;
+    return k8_tiles(K8_BIG, m, n) >= 256 ? K8_BIG : K8_MIDDLE;
+}
+template <bool I8, class Epi> hipError_t k8_product(G8 g, K8Tiling t, const Epi &e, hipStream_t st) {
+    const int bm = t == K8_BIG ? 256 : 128, bn = t == K8_BIG ? 256 : t == K8_MIDDLE ? 128 : 64;
+    g.tiles_m = (int)((g.m + bm - 1) / bm); g.tiles_n = (int)((g.n + bn - 1) / bn);
+    const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits));
+    if (t == K8_BIG) k8_gemm<I8, 256, 256, 2, 4, Epi><<<grid, 512, 0, st>>>(g, e);
+    else if (t == K8_MIDDLE) k8_gemm<I8, 128, 128, 2, 2, Epi><<<grid, 256, 0, st>>>(g, e);
+    else k8_gemm<I8, 128, 64, 4, 1, Epi><<<grid, 256, 0, st>>>(g, e);
+    return hipGetLastError();
+}

@@ -937,7 +937,7 @@ __global__ __launch_bounds__(1024) void k8_dw_join(const float *__restrict__ par
 
 // ---- which way a call takes.  Nothing here looks at which results are asked for: a result's bits do not depend on its company -----------------------------------------
 struct Plan {
-    bool few = false, narrow = false, big = false; int dx_splits = 1, np_x = 1, np_w = 1, pitch = 0;
+    bool few = false, narrow = false; K8Tiling tile = K8_BIG; int dx_splits = 1, np_x = 1, np_w = 1, pitch = 0;
     int s = 256, tiles_n = 1, tiles_k = 1, splits = 1; int64_t run = 0;
     uint64_t pieces = 0, turned = 0, down = 0, dx_part = 0, part = 0, part_b = 0, total = 0;
 };
@@ -958,10 +958,10 @@ Plan plan_grad(const dn_i8_grad_desc &d) {
         p.pieces = take((uint64_t)p.np_x * d.m * p.pitch * 2);
         p.turned = take((uint64_t)d.k * p.pitch * 2);
         p.down = take((uint64_t)d.m * 4);
-        const int64_t t256 = ((d.m + 255) / 256) * ((d.k + 255) / 256), t128 = ((d.m + 127) / 128) * ((d.k + 127) / 128), steps = (p.pitch * 2 + 127) / 128 * p.np_x;
-        p.big = t256 >= K8_CUS && d.k > 64;
-        if (!p.big && t128 < K8_CUS) {
-            p.dx_splits = (int)std::max<int64_t>(1, std::min<int64_t>(K8_CUS / t128, steps / 4));
+        p.tile = k8_tiling(d.m, d.k);
+        const int64_t tiles = k8_tiles(p.tile, d.m, d.k), steps = (p.pitch * 2 + 127) / 128 * p.np_x;
+        if (tiles < K8_CUS) {
+            p.dx_splits = (int)std::max<int64_t>(1, std::min<int64_t>(K8_CUS / tiles, steps / 4));
             if (p.dx_splits > 1) p.dx_part = take((uint64_t)p.dx_splits * d.m * d.k * 4);
         }
     }
@@ -995,15 +995,8 @@ Plan plan_grad(const dn_i8_grad_desc &d) {
 }
 
 template <class T, int NP, class Epi> hipError_t dx_gemm(const dn_i8_grad_desc &d, const Plan &p, char *base, const Epi &e, hipStream_t st) {
-    const int b = p.big ? 256 : 128, bk = p.big || d.k > 64 ? b : 64;
     const int64_t plane = d.m * (int64_t)p.pitch * 2;
-    G8 g = { base + p.pieces, base + p.turned, (int64_t)p.pitch * 2, (int64_t)p.pitch * 2, d.m, d.k, p.pitch * 2, NP, plane, p.dx_splits,
-             (int)((d.m + b - 1) / b), (int)((d.k + bk - 1) / bk) };
-    const unsigned grid = (unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits);
-    if (bk == 64) k8_gemm<false, 128, 64, 4, 1, Epi><<<dim3(grid), 256, 0, st>>>(g, e);
-    else if (p.big) k8_gemm<false, 256, 256, 2, 4, Epi><<<dim3(grid), 512, 0, st>>>(g, e);
-    else k8_gemm<false, 128, 128, 2, 2, Epi><<<dim3(grid), 256, 0, st>>>(g, e);
-    return hipGetLastError();
+    return k8_product<false>(G8{ base + p.pieces, base + p.turned, (int64_t)p.pitch * 2, (int64_t)p.pitch * 2, d.m, d.k, p.pitch * 2, NP, plane, p.dx_splits, 0, 0 }, p.tile, e, st);
 }
 template <class T, int NP> hipError_t dx_of(const dn_i8_grad_desc &d, const Plan &p, char *base, hipStream_t st) {
     if (p.few) {
