@@ -101,16 +101,14 @@ template <class T>
 hipError_t rows_of(int64_t m, int k, const T *x, int64_t ldx, int8_t *q, int64_t ldq, float *s, hipStream_t st) {
     constexpr int E = 16 / sizeof(T);
 #define ROWS(LPR_, V_, R_) k8_rows_k<T, LPR_, V_, R_><<<dim3((unsigned)((m + (256 / LPR_) * R_ - 1) / ((256 / LPR_) * R_))), 256, 0, st>>>(m, k, x, ldx, q, ldq, s)
-    // a wavefront or less per row where there are rows enough to fill the chip that way; a workgroup per row for few or long rows
-    const bool many = m >= 8 * K8_CUS;
+    // a wavefront or less per row up to 128 pieces of 16 bytes, if there are rows enough to fill the chip that way; a workgroup per row for few or long rows.  Rows and back,
+    // bf16, us, wavefront : workgroup -- 200000 x 1000, 224 : 304; 100000 x 600, 67 : 119; 100 x 1000, 7.1 : 5.7; 8192 x 4096, 37 : 33; 2048 x 4096, 11.9 : 10.5
     const int pieces = (k + E - 1) / E;
     if (pieces <= 8) ROWS(8, 1, 4);
     else if (pieces <= 16) ROWS(16, 1, 4);
     else if (pieces <= 32) ROWS(32, 1, 4);
     else if (pieces <= 64) ROWS(64, 1, 4);
-    else if (pieces <= 128 && many) ROWS(64, 2, 2);
-    else if (pieces <= 256 && many) ROWS(64, 4, 1);
-    else if (pieces <= 512 && many) ROWS(64, 8, 1);
+    else if (pieces <= 128 && m >= 8 * K8_CUS) ROWS(64, 2, 2);
     else if (pieces <= 256) ROWS(256, 1, 1);
     else if (pieces <= 512) ROWS(256, 2, 1);
     else if (pieces <= 1024) ROWS(256, 4, 1);
@@ -160,7 +158,7 @@ hipError_t restore_of(int64_t m, int k, const int8_t *q, int64_t ldq, const floa
     else if (pieces <= 16) REST(16, 4);
     else if (pieces <= 32) REST(32, 4);
     else if (pieces <= 64 && m >= 8 * K8_CUS) REST(64, 4);
-    else if (m >= 8 * K8_CUS) REST(64, 1);
+    else if (pieces <= 128 && m >= 8 * K8_CUS) REST(64, 1);
     else REST(256, 1);
 #undef REST
     return hipGetLastError();
@@ -451,17 +449,33 @@ __global__ __launch_bounds__(512) void k8_narrow(const X *__restrict__ x, int64_
     const int lane = threadIdx.x & 63, wave = k8_uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.y * 256;
     const int cols = (int)min((int64_t)256, o.n - n0), blocks = (cols + 63) / 64;
+#pragma unroll 4
     for (int f = threadIdx.x; f < blocks * 4 * KS * 64; f += 512) {
         const int fl = f & 63, ks = (f >> 6) % KS, t = (f >> 6) / KS % 4, blk = (f >> 6) / (KS * 4);
         const int col = blk * 64 + 4 * (fl & 15) + t;
-        K8Vec<int8_t, 16> v;
         const int8_t *wr = w + (n0 + min(col, cols - 1)) * ldw;
+        // runs of C codes; one that ends behind the row is read in front of its end and moved down.  No branch around a load: it would be waited for there
+        constexpr int C = E < 8 ? E : 8;
+        uint64_t v[16 / C];
 #pragma unroll
-        for (int b = 0; b < 16; b++) {
-            const int kk = k8_piece_of<X>(ks, fl >> 4, b);
-            v.v[b] = col < cols && kk < k ? wr[kk] : (int8_t)0;
+        for (int j = 0; j < 16 / C; j++) {
+            const int at = k8_piece_of<X>(ks, fl >> 4, j * C), from = min(at, k - C);
+            v[j] = 0;
+            if (k >= C) __builtin_memcpy(&v[j], wr + from, C);
+            else
+#pragma unroll
+                for (int b = 0; b < C; b++) v[j] |= (uint64_t)(uint8_t)wr[min(b, k - 1)] << (8 * b);
         }
-        *(i32x4 *)(lw + f * 16) = __builtin_bit_cast(i32x4, v);
+        i32x4 out;
+#pragma unroll
+        for (int j = 0; j < 16 / C; j++) {
+            const int at = k8_piece_of<X>(ks, fl >> 4, j * C), skip = k >= C ? min(max(at + C - k, 0), C) : 0, have = k >= C ? C : max(k - at, 0);
+            uint64_t r = skip < 8 ? v[j] >> (8 * skip) : 0;
+            if (have < C) r &= (1ull << (8 * have)) - 1;
+            out[j * C / 4] = (int)(unsigned)r;
+            if (C == 8) out[(j * C / 4 + 1) & 3] = (int)(unsigned)(r >> 32);
+        }
+        *(i32x4 *)(lw + f * 16) = out;
     }
     for (int i = threadIdx.x; i < 256; i += 512) {
         lsw[i] = i < cols ? o.sw[n0 + i] : 0.0f;
@@ -580,9 +594,14 @@ Plan plan_linear(const dn_i8_linear_desc &d) {
     Plan p;
     const bool given = d.x_type == DN_T_I8;
     auto take = [&](uint64_t bytes) { const uint64_t at = p.total; p.total += k8_up(bytes, 256); return at; };
+    // few rows: one launch (or two) without tiles of 128 rows.  us, this : tiles, bf16, 4096 x 4096 -- 17 rows, 10 : 15; 64 rows, 16 : 17; 64 x 1000 x 1000, 11 : 13
     if (d.m <= 64) p.way = FEW;
-    else if (d.k <= 256 && d.n <= 512 && (given || d.x_type == d.y_type)) { p.way = NARROW; return p; }
-    // few rows of numbers: their codes fit a workgroup's LDS beside its sums
+    // Narrow rows: one launch that reads x once, but every workgroup first lays out its 256 channels of the weight (K > 128: 10 us).  us, this : rows and tiles, bf16 --
+    // 200 x 64 x 64, 5.7 : 9.8; 100000 x 64 x 512, 41 : 73; 20000 x 128 x 2048, 47 : 56; 5000 x 256 x 256, 17 : 12; 50000 x 256 x 256, 34 : 35; 1048576 x 256 x 256, 383 : 475;
+    // 20000 x 256 x 512, 35 : 29; 20000 x 256 x 1024, 42 : 46
+    else if ((given || d.x_type == d.y_type) && (d.k <= 128 ? d.n <= 2048 : d.k <= 256 && d.n <= 1024 && d.m * ((d.n + 255) / 256) >= 49152)) { p.way = NARROW; return p; }
+    // few rows of numbers: their codes fit a workgroup's LDS beside its sums.  That saves a launch and a workspace (3 us of a call); on the device alone it costs as much
+    // (1 x 4096 x 4096: 8.3 us, in two launches 8.1; 16 x 1024 x 1024: 8.8 and 6.5)
     p.inside = p.way == FEW && !given && d.m <= 16 && d.m * d.k <= 16384;
     if (p.inside) return p;
     if (!given && !d.q) {

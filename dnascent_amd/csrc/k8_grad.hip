@@ -37,6 +37,25 @@ __device__ __forceinline__ void k8_columns(const unsigned (&d)[8], i32x4 (&out)[
             out[j][p] = __builtin_bit_cast(int, __builtin_bit_cast(k8_f16x2, t) - k8_f16x2{ (_Float16)1152.0f, (_Float16)1152.0f });
         }
 }
+// rows nn .. nn + 7 of four codes each from channel kk on, without a branch around a load: rows behind the last one repeat it (what they are multiplied with is zero),
+// four channels that end behind the matrix are read in front of its end and moved down
+__device__ __forceinline__ void k8_eight_rows(const dn_i8_grad_desc &d, int nn, int64_t kk, unsigned (&rows)[8]) {
+    if (d.k >= 4) {
+        const int64_t at = min(kk, d.k - 4);
+        const int skip = 8 * (int)min(kk - at, (int64_t)3);
+#pragma unroll
+        for (int e = 0; e < 8; e++) __builtin_memcpy(&rows[e], d.w + min((int64_t)(nn + e), d.n - 1) * d.ldw + at, 4);
+#pragma unroll
+        for (int e = 0; e < 8; e++) rows[e] >>= skip;
+    } else
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int8_t *p = d.w + min((int64_t)(nn + e), d.n - 1) * d.ldw;
+            rows[e] = 0u;
+#pragma unroll
+            for (int j = 0; j < 4; j++) rows[e] |= (unsigned)(uint8_t)p[min(kk + j, d.k - 1)] << (8 * j);
+        }
+}
 // the power of two that puts `top` (bits of a magnitude, finite) into [2^14, 2^15), and its inverse; both are normal numbers
 struct K8Pow { float up, down; };
 __device__ __forceinline__ K8Pow k8_pow(unsigned top) {
@@ -57,20 +76,11 @@ __global__ __launch_bounds__(WG) void k8_dx_narrow(dn_i8_grad_desc d) {
     const int n = (int)d.n;
     const int64_t k0 = (int64_t)blockIdx.y * 256;
     const int cols = (int)min((int64_t)256, d.k - k0), blocks = (cols + 63) / 64;
+#pragma unroll 2
     for (int f = threadIdx.x; f < blocks * NS * 64; f += WG) {
         const int fc = f & 15, fg = (f >> 4) & 3, step = (f >> 6) % NS, blk = (f >> 6) / NS, kk = blk * 64 + 4 * fc;
         unsigned rows[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int nn = step * 32 + 8 * fg + e;
-            rows[e] = 0;
-            if (nn < n) {
-                const int8_t *wr = d.w + nn * d.ldw + k0 + kk;
-                if (kk + 4 <= cols) __builtin_memcpy(&rows[e], wr, 4);
-                else
-                    for (int b = 0; b < 4; b++) if (kk + b < cols) rows[e] |= (unsigned)(uint8_t)wr[b] << (8 * b);
-            }
-        }
+        k8_eight_rows(d, step * 32 + 8 * fg, k0 + kk, rows);
         i32x4 out[4];
         k8_columns(rows, out);
 #pragma unroll
@@ -220,31 +230,38 @@ __global__ __launch_bounds__(WG) void k8_dx_narrow(dn_i8_grad_desc d) {
 }
 
 // ---- dx, wide layers: the pieces of dz sw as rows of fp16, the transposed weight as rows of fp16, then k8_gemm -----------------------------------------------------
-// LPR lanes walk a row twice (the second time from cache).  np: pitch in fp16, a multiple of 8; zeros behind n
-template <class T, int LPR, int NP>
+// LPR lanes hold a row, V pieces of eight numbers each; with V = 0 they walk it twice (the second time from cache).  np: pitch in fp16, a multiple of 8; zeros behind n
+template <class T, int LPR, int V, int NP>
 __global__ __launch_bounds__(256) void k8_pieces(dn_i8_grad_desc d, _Float16 *__restrict__ out, int np, int64_t plane, float *__restrict__ down) {
     const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
     const int lid = threadIdx.x % LPR, n = (int)d.n;
     const int64_t rr = min(row, d.m - 1);
     const T *p = (const T *)d.dy + rr * d.ldy;
     const uint8_t *mk = d.mask ? d.mask + rr * d.ldmask : nullptr;
-    float v[8];
-    auto piece = [&](int at) {
-        const unsigned bits = mk ? mk[at >> 3] : 255u;
-        K8Vec<T, 8> x; K8Vec<float, 8> sw;
-        if (at + 8 <= n) { x = k8_load<T, 8>(p + at); sw = k8_load<float, 8>(d.sw + at); }
-        else
+    constexpr int HELD = V ? V : 1;
+    K8Raw<T, 8> x[HELD]; K8Raw<float, 8> sw[HELD]; unsigned bits[HELD];
+    float v[HELD][8];
+    auto load = [&](int i, int at) __attribute__((always_inline)) {            // zeros behind the row's end
+        if (at + 8 <= n) { x[i].load(p + at); sw[i].load(d.sw + at); }
+        else { x[i].load(p + at, n - at); sw[i].load(d.sw + at, n - at); }
+        bits[i] = mk ? mk[min(at, n - 1) >> 3] : 255u;
+    };
+    auto make = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) { x.v[e] = at + e < n ? p[at + e] : (T)0.0f; sw.v[e] = at + e < n ? d.sw[at + e] : 0.0f; }
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = (bits >> e & 1 ? (float)x.v[e] : 0.0f) * sw.v[e];
+        for (int e = 0; e < 8; e++) v[i][e] = __uint_as_float(__float_as_uint(x[i].get(e)) & (unsigned)((int)(bits[i] << (31 - e)) >> 31)) * sw[i].get(e);
     };
     unsigned top = 0;
-    for (int at = lid * 8; at < n; at += LPR * 8) {
-        piece(at);
+    auto most = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) { const unsigned b = k8_mag(v[e]); top = max(top, b < 0x7f800000u ? b : 0u); }
-    }
+        for (int e = 0; e < 8; e++) { const unsigned b = k8_mag(v[i][e]); top = max(top, b < 0x7f800000u ? b : 0u); }
+    };
+    if (V) {
+#pragma unroll
+        for (int i = 0; i < V; i++) load(i, (i * LPR + lid) * 8);
+#pragma unroll
+        for (int i = 0; i < V; i++) { make(i); most(i); }
+    } else
+        for (int at = lid * 8; at < n; at += LPR * 8) { load(0, at); make(0); most(0); }
 #pragma unroll
     for (int o = (LPR < 64 ? LPR : 64) / 2; o; o >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, o));
     if (LPR == 256) {
@@ -256,40 +273,33 @@ __global__ __launch_bounds__(256) void k8_pieces(dn_i8_grad_desc d, _Float16 *__
     if (row >= d.m) return;
     const K8Pow pw = k8_pow(top);
     if (lid == 0) down[row] = pw.down;
-    for (int at = lid * 8; at < np; at += LPR * 8) {
+    auto store = [&](int i, int at) __attribute__((always_inline)) {
         i32x4 hi, lo;
-        if (at < n) piece(at);
-        else
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = 0.0f;
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            const K8Split w = k8_split(v[2 * q] * pw.up, v[2 * q + 1] * pw.up);
-            hi[q] = w.hi; lo[q] = w.lo;
+            const float v0 = v[i][2 * q] * pw.up, v1 = v[i][2 * q + 1] * pw.up;
+            if (NP == 2) { const K8Split w = k8_split(v0, v1); hi[q] = w.hi; lo[q] = w.lo; }
+            else hi[q] = k8_pack(v0, v1);
         }
         *(i32x4 *)(out + row * np + at) = hi;
         if (NP == 2) *(i32x4 *)(out + plane + row * np + at) = lo;
-    }
+    };
+    if (V) {
+#pragma unroll
+        for (int i = 0; i < V; i++) if ((i * LPR + lid) * 8 < np) store(i, (i * LPR + lid) * 8);
+    } else
+        for (int at = lid * 8; at < np; at += LPR * 8) { load(0, at); make(0); store(0, at); }
 }
 // w [n][k] codes -> [k][np] fp16, zeros behind n.  A thread takes 8 n x 4 k; the 8 lanes beside it the next 64 n
 __global__ __launch_bounds__(256) void k8_turn(dn_i8_grad_desc d, _Float16 *__restrict__ out, int np) {
-    const int n = (int)d.n, k = (int)d.k;
+    const int k = (int)d.k;
     const int64_t nb = (np + 63) / 64, kb = (k + 127) / 128;
     const int64_t bn = blockIdx.x % nb, bk = blockIdx.x / nb;
     if (bk >= kb) return;
     const int nn = (int)bn * 64 + (threadIdx.x & 7) * 8, kk = (int)bk * 128 + (threadIdx.x >> 3) * 4;
     if (nn >= np || kk >= k) return;
     unsigned rows[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        rows[e] = 0;
-        if (nn + e < n) {
-            const int8_t *wr = d.w + (int64_t)(nn + e) * d.ldw + kk;
-            if (kk + 4 <= k) __builtin_memcpy(&rows[e], wr, 4);
-            else
-                for (int b = 0; b < 4; b++) if (kk + b < k) rows[e] |= (unsigned)(uint8_t)wr[b] << (8 * b);
-        }
-    }
+    k8_eight_rows(d, nn, kk, rows);
     i32x4 o[4];
     k8_columns(rows, o);
 #pragma unroll
@@ -946,8 +956,12 @@ Plan plan_grad(const dn_i8_grad_desc &d) {
     auto take = [&](uint64_t bytes) { const uint64_t at = p.total; p.total += k8_up(bytes, 256); return at; };
     p.np_x = d.dy_type == DN_T_F32 ? 2 : 1;
     p.np_w = d.dw_type == DN_T_F32 ? 2 : 1;
+    // us, dx and dw, bf16, few : tiles -- 16 x 1024 x 1024, 14 : 27; 16 x 4096 x 4096, 32 : 55; 1 x 64 x 64, 9 : 18
     p.few = d.m >= 1 && d.m <= 16 && d.k >= 4;
-    p.narrow = d.n <= 256 && d.k <= 1024;
+    // one launch that reads dy once for 256 input channels, behind a weight that every workgroup lays out first.  us, dx and dw, bf16, this : pieces and tiles (M x K x N) --
+    // 8000 x 64 x 64, 21 : 29; 100 x 1024 x 128, 21 : 23; 5000 x 4096 x 64, 43 : 61; 300 x 256 x 256, 31 : 26; 2000 x 1024 x 256, 41 : 37; 50000 x 256 x 256, 67 : 83;
+    // 50000 x 2048 x 200, 184 : 264
+    p.narrow = d.k <= 4096 && (d.n <= 128 || (d.n <= 256 && d.m * ((d.k + 255) / 256) >= 16384));
     if (p.few) {
         p.dx_splits = (int)std::max<int64_t>(1, std::min<int64_t>(K8_CUS / ((d.k + 63) / 64), d.n / 1024));
         if (d.dx && p.dx_splits > 1) p.dx_part = take((uint64_t)p.dx_splits * d.m * d.k * 4);
@@ -1018,8 +1032,14 @@ template <class T, int NP> hipError_t dx_of(const dn_i8_grad_desc &d, const Plan
     _Float16 *pieces = (_Float16 *)(base + p.pieces), *turned = (_Float16 *)(base + p.turned);
     float *down = (float *)(base + p.down);
     const int64_t plane = d.m * (int64_t)p.pitch;
-    if (d.n <= 2048 && d.m >= 4 * K8_CUS) k8_pieces<T, 64, NP><<<dim3((unsigned)((d.m + 3) / 4)), 256, 0, st>>>(d, pieces, p.pitch, plane, down);
-    else k8_pieces<T, 256, NP><<<dim3((unsigned)d.m), 256, 0, st>>>(d, pieces, p.pitch, plane, down);
+#define PIECES(LPR_, V_) k8_pieces<T, LPR_, V_, NP><<<dim3((unsigned)((d.m + 256 / LPR_ - 1) / (256 / LPR_))), 256, 0, st>>>(d, pieces, p.pitch, plane, down)
+    if (d.n <= 512) PIECES(64, 1);
+    else if (d.n <= 1024) PIECES(64, 2);
+    else if (d.n <= 2048) PIECES(64, 4);
+    else if (d.n <= 4096) PIECES(256, 2);
+    else if (d.n <= 8192) PIECES(256, 4);
+    else PIECES(256, 0);
+#undef PIECES
     k8_turn<<<dim3((unsigned)(((p.pitch + 63) / 64) * ((d.k + 127) / 128))), 256, 0, st>>>(d, turned, p.pitch);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -1045,7 +1065,9 @@ template <class T, int NP> hipError_t dw_of(const dn_i8_grad_desc &d, const Plan
     else if (p.s == 128) k8_dw<T, 128, NP><<<grid, 512, 0, st>>>(d, o);
     else k8_dw<T, 256, NP><<<grid, 512, 0, st>>>(d, o);
     if (p.splits > 1) {
-        const int64_t each = p.splits > 32 && d.n * d.k < 1024 * K8_CUS ? 256 : 1024;
+        // many runs of few results: their loads shared by sixteen wavefronts (200000 x 64 x 64, 44.1 us: 47.0 without), else four results of all runs per lane
+        // (5000 x 256 x 256, 34 us: 43 the other way; 7552 x 1664 x 1216, 82: 169)
+        const int64_t each = p.splits > 32 && d.n * d.k < 128 * K8_CUS ? 256 : 1024;
         const unsigned dw_blocks = d.dw ? (unsigned)((d.n * d.k + each - 1) / each) : 0, db_blocks = d.db ? (unsigned)((d.n + each - 1) / each) : 0;
         if (each == 1024) k8_dw_join_few<<<dim3(dw_blocks + db_blocks), 256, 0, st>>>(o.part, o.part_b, p.splits, d.n, d.k, d.dw, d.lddw, d.db, d.dw_type, dw_blocks);
         else k8_dw_join<<<dim3(dw_blocks + db_blocks), 1024, 0, st>>>(o.part, o.part_b, p.splits, d.n, d.k, d.dw, d.lddw, d.db, d.dw_type, dw_blocks);
