@@ -741,27 +741,26 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
         if (with_q && base == r0) lower_powers(esh);
         tile(std::false_type(), [&]() __attribute__((always_inline)) { fetch(base, std::false_type()); }, []() {});
     }
-    // ---- the sums leave: sets of wavefronts joined in LDS first, in the order of the sets
+    // ---- the sums leave: sets of wavefronts joined in LDS first, half of the sets to the other half
     __syncthreads();
     const bool last = o.splits == 1;
     if (with_q) {
-        float *js = (float *)lds;                          // [blocks][4 * TK * 4][64] floats
-        if (D::SETS > 1)
-            for (int s = 1; s < D::SETS; s++) {
-                if (set == s)
+        float *js = (float *)lds;                          // [sets / 2][blocks][4 * TK][64] x 4 floats
+        static_assert((D::SETS & (D::SETS - 1)) == 0 && D::SETS / 2 * D::BLOCKS * 4 * TK * 1024 <= 2 * D::LDS, "half of the sets' sums fit the stages");
+        for (int half = D::SETS / 2; half; half /= 2) {
+            if (set >= half && set < 2 * half)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
+                for (int i = 0; i < 4; i++)
 #pragma unroll
-                        for (int j = 0; j < TK; j++)
-                            *(k8_f32x4 *)(js + ((block * 4 + i) * TK + j) * 256 + lane * 4) = acc[i][j];
-                __syncthreads();
-                if (set == 0)
+                    for (int j = 0; j < TK; j++) *(k8_f32x4 *)(js + ((((set - half) * D::BLOCKS + block) * 4 + i) * TK + j) * 256 + lane * 4) = acc[i][j];
+            __syncthreads();
+            if (set < half)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
+                for (int i = 0; i < 4; i++)
 #pragma unroll
-                        for (int j = 0; j < TK; j++) acc[i][j] += *(const k8_f32x4 *)(js + ((block * 4 + i) * TK + j) * 256 + lane * 4);
-                __syncthreads();
-            }
+                    for (int j = 0; j < TK; j++) acc[i][j] += *(const k8_f32x4 *)(js + (((set * D::BLOCKS + block) * 4 + i) * TK + j) * 256 + lane * 4);
+            __syncthreads();
+        }
         if (set == 0)
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -1067,7 +1066,7 @@ template <class T, int NP> hipError_t dw_of(const dn_i8_grad_desc &d, const Plan
     if (p.splits > 1) {
         // many runs of few results: their loads shared by sixteen wavefronts (200000 x 64 x 64, 44.1 us: 47.0 without), else four results of all runs per lane
         // (5000 x 256 x 256, 34 us: 43 the other way; 7552 x 1664 x 1216, 82: 169)
-        const int64_t each = p.splits > 32 && d.n * d.k < 128 * K8_CUS ? 256 : 1024;
+        const int64_t each = p.splits > 8 && d.n * d.k < 128 * K8_CUS ? 256 : 1024;
         const unsigned dw_blocks = d.dw ? (unsigned)((d.n * d.k + each - 1) / each) : 0, db_blocks = d.db ? (unsigned)((d.n + each - 1) / each) : 0;
         if (each == 1024) k8_dw_join_few<<<dim3(dw_blocks + db_blocks), 256, 0, st>>>(o.part, o.part_b, p.splits, d.n, d.k, d.dw, d.lddw, d.db, d.dw_type, dw_blocks);
         else k8_dw_join<<<dim3(dw_blocks + db_blocks), 1024, 0, st>>>(o.part, o.part_b, p.splits, d.n, d.k, d.dw, d.lddw, d.db, d.dw_type, dw_blocks);
