@@ -627,13 +627,21 @@ Plan plan_linear(const dn_i8_linear_desc &d) {
                      default: { typedef k8_bf16 T_; __VA_ARGS__; break; } }
 
 hipError_t k8_rows(int64_t m, int64_t k, const void *x, int64_t ldx, int x_type, int8_t *q, int64_t ldq, float *s, hipStream_t st) {
-    if (m == 0) return hipSuccess;
-    K8_TYPE(x_type, T, return rows_of<T>(m, (int)k, (const T *)x, ldx, q, ldq, s, st));
+    for (int64_t r = 0; r < m; r += K8_LAUNCH_ROWS) {
+        hipError_t e = hipSuccess;
+        K8_TYPE(x_type, T, e = rows_of<T>(std::min(m - r, K8_LAUNCH_ROWS), (int)k, (const T *)x + r * ldx, ldx, q + r * ldq, ldq, s + r, st));
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 hipError_t k8_restore(int64_t m, int64_t k, const int8_t *q, int64_t ldq, const float *s, void *x, int64_t ldx, int x_type, hipStream_t st) {
-    if (m == 0) return hipSuccess;
-    K8_TYPE(x_type, T, return restore_of<T>(m, (int)k, q, ldq, s, (T *)x, ldx, st));
+    for (int64_t r = 0; r < m; r += K8_LAUNCH_ROWS) {
+        hipError_t e = hipSuccess;
+        K8_TYPE(x_type, T, e = restore_of<T>(std::min(m - r, K8_LAUNCH_ROWS), (int)k, q + r * ldq, ldq, s + r, (T *)x + r * ldx, ldx, st));
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 uint64_t k8_linear_workspace(const dn_i8_linear_desc &d) { return plan_linear(d).total; }

@@ -14,6 +14,8 @@ template <class T, int N> __device__ __forceinline__ void k8_store(T *p, const K
 typedef unsigned __attribute__((ext_vector_type(2), aligned(1))) k8_u32x2;
 typedef unsigned __attribute__((ext_vector_type(4), aligned(1))) k8_u32x4;
 typedef unsigned __attribute__((aligned(1))) k8_u32;
+// rows of one launch where a workgroup or wavefront has a row: a grid holds fewer than 2^32 threads
+constexpr int64_t K8_LAUNCH_ROWS = 1 << 23;
 // results that are not read again soon: past the caches
 template <class T, int N> __device__ __forceinline__ void k8_stream(T *p, const K8Vec<T, N> &v) {
     if constexpr (sizeof v == 16) { k8_u32x4 w; __builtin_memcpy(&w, &v, 16); __builtin_nontemporal_store(w, (k8_u32x4 *)p); }

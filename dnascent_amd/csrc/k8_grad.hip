@@ -1031,14 +1031,20 @@ template <class T, int NP> hipError_t dx_of(const dn_i8_grad_desc &d, const Plan
     _Float16 *pieces = (_Float16 *)(base + p.pieces), *turned = (_Float16 *)(base + p.turned);
     float *down = (float *)(base + p.down);
     const int64_t plane = d.m * (int64_t)p.pitch;
-#define PIECES(LPR_, V_) k8_pieces<T, LPR_, V_, NP><<<dim3((unsigned)((d.m + 256 / LPR_ - 1) / (256 / LPR_))), 256, 0, st>>>(d, pieces, p.pitch, plane, down)
-    if (d.n <= 512) PIECES(64, 1);
-    else if (d.n <= 1024) PIECES(64, 2);
-    else if (d.n <= 2048) PIECES(64, 4);
-    else if (d.n <= 4096) PIECES(256, 2);
-    else if (d.n <= 8192) PIECES(256, 4);
-    else PIECES(256, 0);
+    for (int64_t r = 0; r < d.m; r += K8_LAUNCH_ROWS) {
+        dn_i8_grad_desc t = d;
+        t.m = std::min(d.m - r, K8_LAUNCH_ROWS);
+        t.dy = (const T *)d.dy + r * d.ldy;
+        if (d.mask) t.mask = d.mask + r * d.ldmask;
+#define PIECES(LPR_, V_) k8_pieces<T, LPR_, V_, NP><<<dim3((unsigned)((t.m + 256 / LPR_ - 1) / (256 / LPR_))), 256, 0, st>>>(t, pieces + r * p.pitch, p.pitch, plane, down + r)
+        if (d.n <= 512) PIECES(64, 1);
+        else if (d.n <= 1024) PIECES(64, 2);
+        else if (d.n <= 2048) PIECES(64, 4);
+        else if (d.n <= 4096) PIECES(256, 2);
+        else if (d.n <= 8192) PIECES(256, 4);
+        else PIECES(256, 0);
 #undef PIECES
+    }
     k8_turn<<<dim3((unsigned)(((p.pitch + 63) / 64) * ((d.k + 127) / 128))), 256, 0, st>>>(d, turned, p.pitch);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

@@ -731,3 +731,24 @@ def test_layer_refusals(ctx):
     i = next(j for j, op in enumerate(desc["ops"]) if op["op"] == "conv" and op["k"] == 1)
     with pytest.raises(ValueError):
         layer.store(desc, blob, i)
+
+
+def test_more_rows_than_one_launch_has(ctx):
+    m, k = 2 ** 23 + 5, 3
+    x = torch.randn(m, k, generator=gen(51), device="cuda").to(BF16)
+    q, s = ctx.i8_rows(x)
+    y = ctx.i8_restore(q, s, BF16)
+    for part in (slice(0, 3), slice(2 ** 23 - 3, m)):
+        qr, sr = codes(x[part])
+        assert np.array_equal(q[part].cpu().numpy(), qr) and s[part].cpu().numpy().tobytes() == sr.tobytes()
+        want = torch.from_numpy(qr).double() * torch.from_numpy(sr).double()[:, None]
+        within(y[part], want, want.abs(), BF16, 2.0 ** -24)
+    n = 257                                                # dx of a wide layer: rows of dz sw first
+    wq, ws = eight(n, k, 52)
+    dy = torch.zeros(m, n, dtype=BF16, device="cuda")
+    at = torch.tensor([0, 1, 2 ** 23 - 1, 2 ** 23, m - 1], device="cuda")
+    dy[at] = torch.randn(5, n, generator=gen(53), device="cuda").to(BF16)
+    dx, _, _ = ctx.i8_linear_grad(dy, q, s, wq, ws, need_dw=False, need_db=False)
+    (want, _, _), (t, _, _) = grad_ref(dy[at], q[at], s[at], wq, ws, None)
+    within(dx[at], want, t, BF16, 2.0 ** -11 + n * 2.0 ** -24)
+    assert int((dx != 0).any(1).sum()) == 5
