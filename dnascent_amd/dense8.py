@@ -7,6 +7,7 @@ The reference has no counterpart: its network is a frozen SavedModel (tensor.cpp
 
 (The wrappers are written for short calls: a small layer's kernel takes a few microseconds, as much as a handful of Python attribute look-ups.)
 """
+import copy
 import ctypes as C
 from typing import NamedTuple, Optional
 
@@ -257,6 +258,13 @@ class Dense(torch.nn.Module):
         self.ctx, self.relu = ctx, bool(relu)
         self.weight = torch.nn.Parameter((torch.randn(n, k, device=device) * k ** -0.5).to(dtype))
         self.bias = torch.nn.Parameter(torch.zeros(n, dtype=dtype, device=device)) if bias else None
+
+    def __deepcopy__(self, memo):
+        memo[id(self.ctx)] = self.ctx                      # parameters of its own, the same device context
+        new = type(self).__new__(type(self))
+        memo[id(self)] = new
+        new.__dict__.update(copy.deepcopy(self.__dict__, memo))
+        return new
 
     def forward(self, x, residual=None):
         return _Layer.apply(x, self.weight, self.bias, residual, self.ctx, self.relu)

@@ -752,3 +752,28 @@ def test_more_rows_than_one_launch_has(ctx):
     (want, _, _), (t, _, _) = grad_ref(dy[at], q[at], s[at], wq, ws, None)
     within(dx[at], want, t, BF16, 2.0 ** -11 + n * 2.0 ** -24)
     assert int((dx != 0).any(1).sum()) == 5
+
+
+def test_layer_copied_one_row_and_state(ctx):
+    import copy
+
+    from dnascent_amd import dense8
+    layer = dense8.Dense(ctx, 40, 24, relu=True)
+    twin = copy.deepcopy(torch.nn.Sequential(layer))[0]
+    assert twin.ctx is ctx and torch.equal(twin.weight, layer.weight) and twin.weight.data_ptr() != layer.weight.data_ptr()
+    x = torch.randn(40, device="cuda").requires_grad_()    # no leading dimension at all
+    res = torch.randn(24, device="cuda").requires_grad_()
+    y = layer(x, res)
+    assert y.shape == (24,) and torch.equal(y, layer(x[None], res[None])[0])
+    y.sum().backward()
+    assert x.grad.shape == (40,) and torch.equal(res.grad, (y > 0).float())
+    with torch.no_grad():
+        twin.weight.zero_()
+    twin.load_state_dict(layer.state_dict())
+    assert torch.equal(twin(x, res), y)
+    other = layer(x)                                       # the weight may change between the passes: what was multiplied is what is differentiated
+    want, = torch.autograd.grad(layer(x).sum(), x)
+    with torch.no_grad():
+        layer.weight.mul_(3)
+    got, = torch.autograd.grad(other.sum(), x)
+    assert torch.equal(got, want)
