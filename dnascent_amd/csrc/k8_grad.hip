@@ -66,7 +66,8 @@ __device__ __forceinline__ K8Pow k8_pow(unsigned top) {
 // ---- dx, narrow layers (N <= 256) ------------------------------------------------------------------------------------------------------------------------------
 // The same shape as the forward pass over narrow rows (k8_narrow): a wavefront takes 16 rows of dy, holds them in registers in the matrix operand's order, finds
 // each row's power of two, and multiplies with the weight, whose transposed fragments lie in LDS as fp16 (256 k x N).  Nothing but dy, the mask and dx moves.
-// NP: pieces.  WG: threads; the weight fills a CU's LDS where N is 256, and what hides the loads is how many wavefronts the registers leave room for
+// NP: pieces.  WG: threads; the weight fills a CU's LDS where N is 256, and what hides the loads is how many wavefronts the registers leave room for.
+// 1 Mi x 256 x 256 bf16 with ReLU: 259 us; its 1.1 GB take 213 at a copy's rate, its products 104, and the vector instructions that mask, scale and convert about as long.
 template <class T, int NS, int NP, int WG>
 __global__ __launch_bounds__(WG) void k8_dx_narrow(dn_i8_grad_desc d) {
     __shared__ __align__(16) char lw[256 * NS * 64];       // fragment (k block of 64, tile t, step) x 64 lanes x 16 bytes: column k = 64 blk + 4 c + t, n = 32 step + 8 g ..
@@ -230,7 +231,8 @@ __global__ __launch_bounds__(WG) void k8_dx_narrow(dn_i8_grad_desc d) {
 }
 
 // ---- dx, wide layers: the pieces of dz sw as rows of fp16, the transposed weight as rows of fp16, then k8_gemm -----------------------------------------------------
-// LPR lanes hold a row, V pieces of eight numbers each; with V = 0 they walk it twice (the second time from cache).  np: pitch in fp16, a multiple of 8; zeros behind n
+// LPR lanes hold a row, V pieces of eight numbers each; with V = 0 they walk it twice (the second time from cache).  np: pitch in fp16, a multiple of 8; zeros behind n.
+// HBM: 8192 x 4096 bf16, 26 us, 5.2 TB/s.  The weight beside it (k8_turn): 4096 x 4096, 14 us; the product: 247 us, 1.11 PFLOP/s.
 template <class T, int LPR, int V, int NP>
 __global__ __launch_bounds__(256) void k8_pieces(dn_i8_grad_desc d, _Float16 *__restrict__ out, int np, int64_t plane, float *__restrict__ down) {
     const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
@@ -376,7 +378,7 @@ __global__ __launch_bounds__(256) void k8_dx_join(const float *__restrict__ part
 // A workgroup takes 64 input channels; its eight wavefronts deal the output channels among themselves, 64 at a time, and join their sums in LDS.  A lane reads
 // eight rows of four codes and makes the operands of the four column tiles of them.  Each 64 numbers of a row have a power of two of their own, so nothing has to
 // be known of a row before the weight's first bytes are asked for.  Where that makes few workgroups for many output channels, the output channels are cut into runs
-// of `run` as well, and k8_dx_join adds the runs' results.
+// of `run` as well, and k8_dx_join adds the runs' results.  Bound by latency: 6 x 1991 x 3807 fp16 11 us, 7 x 16384 x 1024 bf16 9 + 5 us (one run: 54), 12 x 4096 x 4096 9 + 3.
 template <class T, int NP>
 __global__ __launch_bounds__(512) void k8_dx_few(dn_i8_grad_desc d, int run, float *part) {
     __shared__ __align__(16) float sums[8][4][256];
@@ -487,9 +489,9 @@ __global__ __launch_bounds__(512) void k8_dx_few(dn_i8_grad_desc d, int run, flo
 // RT at a time: a thread reads eight rows of four adjacent channels, makes the fp16 values and writes them to LDS turned -- eight rows of one channel are the
 // 16 bytes a matrix instruction takes.  The rows of the next tile are in flight while this one multiplies.
 //
-// Every output channel has a power of two, agreed on by the whole workgroup: it starts so high that the first number which is not tiny does not fit, and whoever
-// sees one that does not fit raises a flag; behind the barrier the workgroup then finds the tile's largest numbers, lowers the powers of the channels that need
-// it (five bits of room), scales their sums so far -- exactly -- and makes the tile again.  That happens for a workgroup's first tile and hardly ever after.
+// Every output channel has a power of two, agreed on by the whole workgroup: it comes from the largest numbers of the first tile, with five bits of room.  Whoever sees
+// a number that does not fit raises a flag; behind the barrier the workgroup then finds that tile's largest numbers, lowers the powers of the channels that need it,
+// scales their sums so far -- exactly -- and makes the tile again, which hardly ever happens.
 //
 // LDS row of a channel: RT rows x 2 bytes (x NP pieces), in pieces of 16 bytes.  Threads that write and lanes that read stand four channels apart: those lie side by side, and
 // sixteen of them reach sixteen different places of the 64 banks.  Wavefronts share the S x S results in blocks of 64 x KB; where there are fewer blocks than wavefronts, sets of wavefronts take turns
@@ -797,6 +799,7 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
 // ---- dw and db, few rows (M <= 16) ------------------------------------------------------------------------------------------------------------------------------
 // dw's bytes are all there is to move.  The factors dz s and the codes go as they are, in fp32, into matrix instructions over four rows; 64 x 64 results per wavefront,
 // tile t of a block holds input channels 4 c + t, so that a lane stores four adjacent ones.  No LDS, no waiting for one another.
+// 6 x 1991 x 3807 fp16 10 us (k8_dw: 24), 12 x 4096 x 4096 bf16 19 us for 34 MB (k8_dw: 20; as fp32 vector products: 22).
 template <class T, class W>
 __global__ __launch_bounds__(256) void k8_dw_few(dn_i8_grad_desc d) {
     const int lane = threadIdx.x & 63, wave = k8_uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4, m = (int)d.m;
@@ -979,9 +982,11 @@ Plan plan_grad(const dn_i8_grad_desc &d) {
         }
     }
     int64_t want = K8_CUS;
-    // dw's tiles and the runs of rows: what costs least, by times measured on whole chips -- a workgroup's row in a tile of 256: 55 ns, of 128: 21; its start and end:
+    // dw's tiles and the runs of rows: what costs least, by times measured on whole chips -- a workgroup's row in a tile of 256: 55 ns (fp16, fp32: 65, their
+    // registers spill), of 128: 21; its start and end:
     // 14 us and 9; a run's results, written and read again: 1.2 ps each.  bf16, us, 256 : 128 -- 1048576 x 256 x 256, 281 : 345; 200000 x 192 x 192, 73 : 89;
-    // 50000 x 1024 x 256, 103 : 85; 7552 x 1664 x 1216, 82 : 139; 1000 x 1024 x 1024, 39 : 23; 64 x 2048 x 4096, 20 : 26
+    // 50000 x 1024 x 256, 103 : 85; 7552 x 1664 x 1216, 82 : 139; 1000 x 1024 x 1024, 39 : 23; 64 x 2048 x 4096, 20 : 26;
+    // fp16, 14400 x 384 x 3028 with dx, 222 : 203; fp32, 100000 x 256 x 256 with dx, 134 : 118
     if (std::max(d.n, d.k) <= 64) p.s = 64;
     else {
         double least = 1e30;
@@ -989,7 +994,7 @@ Plan plan_grad(const dn_i8_grad_desc &d) {
             const int64_t tiles = ((d.n + side - 1) / side) * ((d.k + side - 1) / side), most = std::max<int64_t>(1, (d.m * p.np_w * side + 16383) / 16384);
             for (int rounds = 1; rounds <= 3; rounds++) {
                 const int64_t runs = std::min(most, std::max<int64_t>(1, rounds * K8_CUS / tiles)), turns = (tiles * runs + K8_CUS - 1) / K8_CUS;
-                const double cost = (double)turns * ((side == 256 ? 14e3 : 9e3) + (side == 256 ? 55.0 : 21.0) * (double)(d.m * p.np_w) / (double)runs) +
+                const double cost = (double)turns * ((side == 256 ? 14e3 : 9e3) + (side == 256 ? (d.dy_type == DN_T_BF16 ? 55.0 : 65.0) : 21.0) * (double)(d.m * p.np_w) / (double)runs) +
                                     (runs > 1 ? 3e3 + 1.2e-3 * (double)(runs * d.n * d.k) : 0.0);
                 if (cost < least) { least = cost; p.s = side; want = runs; }
             }
