@@ -66,10 +66,11 @@ __device__ __forceinline__ K8Pow k8_pow(unsigned top) {
 // ---- dx, narrow layers (N <= 256) ------------------------------------------------------------------------------------------------------------------------------
 // The same shape as the forward pass over narrow rows (k8_narrow): a wavefront takes 16 rows of dy, holds them in registers in the matrix operand's order, finds
 // each row's power of two, and multiplies with the weight, whose transposed fragments lie in LDS as fp16 (256 k x N).  Nothing but dy, the mask and dx moves.
-// NP: pieces.  WG: threads; the weight fills a CU's LDS where N is 256, and what hides the loads is how many wavefronts the registers leave room for.
-// 1 Mi x 256 x 256 bf16 with ReLU: 259 us; its 1.1 GB take 213 at a copy's rate, its products 104, and the vector instructions that mask, scale and convert about as long.
-template <class T, int NS, int NP, int WG>
-__global__ __launch_bounds__(WG) void k8_dx_narrow(dn_i8_grad_desc d) {
+// NP: pieces.  512 threads keep everything in registers; 768 hide more but spill (100000 x 256 x 256 with dw, bf16, us: 80 : 91; 1 Mi rows, 499 : 517).
+// 1 Mi x 256 x 256 bf16 with ReLU: 240 us; its 1.1 GB take 213 at a copy's rate, its products 104, and the vector instructions that mask, scale and convert about as long.
+template <class T, int NS, int NP>
+__global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d) {
+    constexpr int WG = 512;
     __shared__ __align__(16) char lw[256 * NS * 64];       // fragment (k block of 64, tile t, step) x 64 lanes x 16 bytes: column k = 64 blk + 4 c + t, n = 32 step + 8 g ..
     __shared__ __align__(16) float lsw[NS * 32];
     __shared__ __align__(16) unsigned keep[sizeof(T) == 2 ? 256 : 1][4];      // a mask byte as eight 16-bit masks
@@ -1026,11 +1027,10 @@ template <class T, int NP> hipError_t dx_of(const dn_i8_grad_desc &d, const Plan
     }
     if (p.narrow) {
         const unsigned per = (unsigned)((d.k + 255) / 256);
-        auto grid = [&](int wg, int each) { return dim3((unsigned)std::min<int64_t>((d.m + wg / 4 - 1) / (wg / 4), each * K8_CUS / per), per); };      // a wavefront has 16 rows
-        constexpr int WIDEST = NP == 1 ? 768 : 512;
-        if (d.n <= 64) k8_dx_narrow<T, 2, NP, 512><<<grid(512, 4), 512, 0, st>>>(d);
-        else if (d.n <= 128) k8_dx_narrow<T, 4, NP, 512><<<grid(512, 2), 512, 0, st>>>(d);
-        else k8_dx_narrow<T, 8, NP, WIDEST><<<grid(WIDEST, 1), WIDEST, 0, st>>>(d);
+        auto grid = [&](int each) { return dim3((unsigned)std::min<int64_t>((d.m + 127) / 128, each * K8_CUS / per), per); };      // a wavefront has 16 rows
+        if (d.n <= 64) k8_dx_narrow<T, 2, NP><<<grid(4), 512, 0, st>>>(d);
+        else if (d.n <= 128) k8_dx_narrow<T, 4, NP><<<grid(2), 512, 0, st>>>(d);
+        else k8_dx_narrow<T, 8, NP><<<grid(1), 512, 0, st>>>(d);
         return hipGetLastError();
     }
     _Float16 *pieces = (_Float16 *)(base + p.pieces), *turned = (_Float16 *)(base + p.turned);
