@@ -67,7 +67,7 @@ __device__ __forceinline__ K8Pow k8_pow(unsigned top) {
 // The same shape as the forward pass over narrow rows (k8_narrow): a wavefront takes 16 rows of dy, holds them in registers in the matrix operand's order, finds
 // each row's power of two, and multiplies with the weight, whose transposed fragments lie in LDS as fp16 (256 k x N).  Nothing but dy, the mask and dx moves.
 // NP: pieces.  512 threads keep everything in registers; 768 hide more but spill (100000 x 256 x 256 with dw, bf16, us: 80 : 91; 1 Mi rows, 499 : 517).
-// 1 Mi x 256 x 256 bf16 with ReLU: 240 us; its 1.1 GB take 213 at a copy's rate, its products 104, and the vector instructions that mask, scale and convert about as long.
+// 1 Mi x 256 x 256 bf16 with ReLU: 252 us; its 1.1 GB take 213 at a copy's rate, its products 104, and the vector instructions that mask, scale and convert about as long.
 template <class T, int NS, int NP>
 __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d) {
     constexpr int WG = 512;
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d) {
 
 // ---- dx, wide layers: the pieces of dz sw as rows of fp16, the transposed weight as rows of fp16, then k8_gemm -----------------------------------------------------
 // LPR lanes hold a row, V pieces of eight numbers each; with V = 0 they walk it twice (the second time from cache).  np: pitch in fp16, a multiple of 8; zeros behind n.
-// HBM: 8192 x 4096 bf16, 26 us, 5.2 TB/s.  The weight beside it (k8_turn): 4096 x 4096, 14 us; the product: 247 us, 1.11 PFLOP/s.
+// HBM: 8192 x 4096 bf16, 22 us, 6.1 TB/s.  The weight beside it (k8_turn): 4096 x 4096, 14 us; the product: 247 us, 1.11 PFLOP/s.
 template <class T, int LPR, int V, int NP>
 __global__ __launch_bounds__(256) void k8_pieces(dn_i8_grad_desc d, _Float16 *__restrict__ out, int np, int64_t plane, float *__restrict__ down) {
     const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
@@ -695,6 +695,8 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 4; j++) pw[j] = power[ch + j];
+#pragma unroll
+        for (int e = 0; e < 8; e++) raw[e].opaque();       // made into numbers again by make(): kept, they would not fit the registers
     };
     // again, next: fetch this tile / the next one
     auto tile = [&](auto whole, auto &&again, auto &&next) __attribute__((always_inline)) {
@@ -720,8 +722,6 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
 #pragma unroll
                         for (int j = 0; j < TK; j++) acc[i][j][q] *= f;
                     }
-#pragma unroll
-                for (int e = 0; e < 8; e++) raw[e].opaque();
                 (void)make(l, std::true_type(), std::false_type());
                 next();
                 __syncthreads();
@@ -983,11 +983,10 @@ Plan plan_grad(const dn_i8_grad_desc &d) {
         }
     }
     int64_t want = K8_CUS;
-    // dw's tiles and the runs of rows: what costs least, by times measured on whole chips -- a workgroup's row in a tile of 256: 55 ns (fp16, fp32: 65, their
-    // registers spill), of 128: 21; its start and end:
-    // 14 us and 9; a run's results, written and read again: 1.2 ps each.  bf16, us, 256 : 128 -- 1048576 x 256 x 256, 281 : 345; 200000 x 192 x 192, 73 : 89;
+    // dw's tiles and the runs of rows: what costs least, by times measured on whole chips -- a workgroup's row in a tile of 256: 55 ns (fp16, fp32: 65), of 128: 21; its start and
+    // end: 14 us and 9; a run's results, written and read again: 1.2 ps each.  bf16, us, 256 : 128 -- 1048576 x 256 x 256, 281 : 345; 200000 x 192 x 192, 73 : 89;
     // 50000 x 1024 x 256, 103 : 85; 7552 x 1664 x 1216, 82 : 139; 1000 x 1024 x 1024, 39 : 23; 64 x 2048 x 4096, 20 : 26;
-    // fp16, 14400 x 384 x 3028 with dx, 222 : 203; fp32, 100000 x 256 x 256 with dx, 134 : 118
+    // with dx, fp16, 12824 x 1088 x 2304, 310 : 338; fp32, 100000 x 256 x 256, 131 : 116
     if (std::max(d.n, d.k) <= 64) p.s = 64;
     else {
         double least = 1e30;
