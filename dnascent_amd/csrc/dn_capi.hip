@@ -136,7 +136,7 @@ struct dn_ctx {
     hipStream_t stream = nullptr;
     bool own_stream = false;
     bool use_dpp = true;
-    std::string err;
+    char err[512] = { 0 };       // the last error's text, in place: the dn_i8_* calls may fail on several threads at once
     size_t dev_bytes = 0;
     // per-batch workspaces come out of grow-only slabs: after the first batches no hipMalloc / hipFree happens per upload
     struct Slab { char *p; size_t cap, used; };
@@ -202,7 +202,7 @@ __attribute__((constructor)) static void dn_runtime_defaults() { setenv("GPU_MAX
 static int fail(dn_ctx *c, int code, const char *fmt, ...) {
     char buf[512];
     va_list ap; va_start(ap, fmt); vsnprintf(buf, sizeof buf, fmt, ap); va_end(ap);
-    if (c) c->err = buf;
+    if (c) memcpy(c->err, buf, strlen(buf) + 1);
     return code;
 }
 #define HIPCHK(c, call)                                                                         \
@@ -499,7 +499,7 @@ void dn_ctx_destroy(dn_ctx *c) {
     delete c;
 }
 
-const char *dn_last_error(const dn_ctx *c) { return c ? c->err.c_str() : "null context"; }
+const char *dn_last_error(const dn_ctx *c) { return c ? c->err : "null context"; }
 
 static int async_status(dn_ctx *c);
 int dn_sync(dn_ctx *c) {

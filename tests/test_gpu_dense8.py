@@ -777,3 +777,33 @@ def test_layer_copied_one_row_and_state(ctx):
         layer.weight.mul_(3)
     got, = torch.autograd.grad(other.sum(), x)
     assert torch.equal(got, want)
+
+
+def test_calls_and_refusals_from_several_threads(ctx):
+    """one context, four threads with a stream each: results as alone, and errors that overlap are errors and nothing worse"""
+    import threading
+    calls = [_mixed(ctx, 900, 256, 256, BF16, 61), _mixed(ctx, 12, 520, 384, F16, 62), _mixed(ctx, 300, 64, 64, F32, 63), _mixed(ctx, 70, 130, 700, BF16, 64)]
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    bad = []
+    d = hip.i8_desc(hip.I8_LINEAR_FIELDS, m=3, n=-5, k=7)
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = calls[i]()
+                    need = C.c_uint64(0)
+                    if hip.lib().dn_i8_linear_workspace(ctx.h, d, C.byref(need)) == 0 or not hip.lib().dn_last_error(ctx.h):
+                        bad.append(("not refused", i))
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        bad.append(("differs", i))
+        except Exception as e:  # noqa: BLE001
+            bad.append((repr(e), i))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad[:4]
