@@ -25,7 +25,7 @@ struct G8 {
     int64_t lda, ldb;
     int64_t m, n;                // rows of a, rows of b
     int kb;                      // bytes of a row that count; i8: any number, fp16: a multiple of 16 (zeros behind the numbers)
-    int planes;                  // the reduction runs over planes of a (plane_a bytes apart) against the same b
+    int planes;                  // the reduction runs over planes of a (plane_a bytes apart) against the same b; two (fp16): the first one's sums count 2^-12
     int64_t plane_a;
     int splits;                  // the reduction is cut into that many runs of steps; run z of a tile is result z
     int tiles_m, tiles_n;
@@ -142,6 +142,17 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k8_gemm(G8 g, Epi epi) {
         }
     };
     // steps go in pairs, one left over goes last.  A step that cuts a row of integers has to be that one: the run then starts a step early, on zeros, if it has to
+    // between the planes: what the first one summed
+    auto lower = [&]() __attribute__((always_inline)) {
+        if constexpr (!I8)
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+#pragma unroll
+                for (int j = 0; j < TN; j++)
+#pragma unroll
+                    for (int q = 0; q < 16; q++) acc[i][j][q] *= 0x1p-12f;
+    };
+    const int border = !I8 && g.planes == 2 ? per_plane : -1;
     const bool cut = I8 && (g.kb & 127) && s1 == steps;
     int s = s0 - (cut && !((s1 - s0) & 1) ? 1 : 0);
     // the next step's loads are asked for in the first two quarters of this one: all at once they keep the wavefronts from their products until the queue has taken
@@ -150,15 +161,19 @@ __global__ __launch_bounds__(64 * WGM * WGN) void k8_gemm(G8 g, Epi epi) {
     if (s < s1) fetch(l0, s, 0, LOADS);
     for (; s + 1 < s1; s += 2) {
         __syncthreads();                                   // this step's loads have landed, and nobody reads the other stage any more
+        if (!I8 && s == border) lower();
         multiply(l0, s, std::false_type(), [&](int q) __attribute__((always_inline)) { fetch(l1, s + 1, q * PER, min(q * PER + PER, LOADS)); });
         __syncthreads();
+        if (!I8 && s + 1 == border) lower();
         const bool more = s + 2 < s1;
         multiply(l1, s + 1, std::false_type(), [&](int q) __attribute__((always_inline)) { if (more) fetch(l0, s + 2, q * PER, min(q * PER + PER, LOADS)); });
     }
     if (s < s1) {
         __syncthreads();
+        if (!I8 && s == border) lower();
         multiply(l0, s, std::true_type(), [](int) {});
     }
+    if (!I8 && s1 <= border) lower();
     // D: column lane & 31, row (q & 3) + 8 (q >> 2) + 4 h.  Lanes outside the matrix stay: an epilogue may put lanes' results together.  What it reads for 16 rows is
     // asked for before the first of them is finished
     const int64_t nn = n0 + wn * TN * 32 + c * TN;

@@ -807,3 +807,42 @@ def test_calls_and_refusals_from_several_threads(ctx):
     for t in threads:
         t.join()
     assert not bad, bad[:4]
+
+
+# ---- results whose own terms are small beside their row's or channel's ------------------------------------------------------------------------------------
+def _outliers(m, n, k, dtype, far, seed):
+    """a few rows of dy are 2^far above the others and a few channels 2^far above those beside them; the codes that stand under them (q's for dw, wq's for dx) are
+    zero in every second column, so that half of the results have small terms only"""
+    dy, q, s, wq, ws, mask = grad_case(m, n, k, F32, seed, True)
+    dy = torch.randn(m, n, generator=gen(seed + 5), device="cuda") * 2.0 ** -8
+    rows_, cols = [0, m // 2, m - 1], [1 % n, n // 2, n - 1]
+    q[rows_, ::2] = 0
+    wq[cols, ::2] = 0
+    by_row, by_col = dy.clone(), dy.clone()
+    by_row[rows_] *= 2.0 ** far
+    by_col[:, cols] *= 2.0 ** far
+    return by_row.to(dtype), by_col.to(dtype), q, s, wq, ws, mask
+
+
+@pytest.mark.parametrize("dtype,w_dtype,far", [(F32, F32, 20), (F32, F32, 36), (F32, F32, 70), (BF16, BF16, 30), (BF16, F32, 60), (F16, F16, 20), (F32, F16, 40)])
+@pytest.mark.parametrize("m,n,k", [(12, 700, 90), (16, 64, 2000), (300, 64, 64), (65, 40, 3), (500, 100, 130), (3000, 256, 256), (40000, 250, 200), (33, 1000, 40), (600, 300, 520),
+                                   (900, 5000, 2), (100, 9000, 70), (70, 1500, 300)])
+def test_grad_of_results_with_small_terms_only(ctx, m, n, k, dtype, w_dtype, far):
+    by_row, by_col, q, s, wq, ws, mask = _outliers(m, n, k, dtype, far, m + n + k)
+    for dy in (by_row, by_col):
+        for mk in (None, mask):
+            got, ref = ctx.i8_linear_grad(dy, q, s, wq, ws, mask=mk, w_dtype=w_dtype), grad_ref(dy, q, s, wq, ws, mk)
+            piece = [2.0 ** -21 if t == F32 else 2.0 ** -11 for t in (dtype, w_dtype)]
+            room = piece[0] + n * 2.0 ** -24, piece[1] + m * 2.0 ** -24, m * 2.0 ** -24               # as check_grad has them
+            check_grad([_border(*v) for v in zip(got, *ref, room)], ref, m, n, dtype, w_dtype)
+
+
+def _border(got, want, terms, u):
+    """Infinity is the right rounding of everything from half a step above the type's largest number on (fp16's largest is 65504, the step there 32: 65520 becomes infinity),
+    so a result that may lie anywhere within its room of `want` may be infinite if want plus room reaches that.  within() only asks for infinity where want minus room
+    is above the largest number; in between both are right, and the largest number (which is within the room) stands in for infinity."""
+    top, half = torch.finfo(got.dtype).max, HALF[got.dtype]
+    want, terms = want.to(got.device), terms.to(got.device)
+    room = half * want.abs() + u * terms
+    near = (want.abs() - room <= top) & (want.abs() + room >= top * (1 + half)) & (got == want.sign() * math.inf)
+    return torch.where(near, (want.sign() * top).to(got.dtype), got)
