@@ -6,6 +6,8 @@
 #include "k8_dense.h"
 
 #include <math.h>
+#include <sys/mman.h>
+#include <unistd.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -1060,17 +1062,31 @@ int dn_host_alloc(size_t bytes, void **p) {
     return hipHostMalloc(p, std::max<size_t>(bytes, 1), hipHostMallocDefault) == hipSuccess ? DN_OK : DN_ERR_HIP;
 }
 void dn_host_free(void *p) { if (p) (void)hipHostFree(p); }
-// Some systems refuse to page-lock memory that exists already.  The arrays then stay pageable: dn_batch_upload asks every pointer what it is and
-// waits for its copies.  The refused pointers are kept so that dn_host_unregister answers for them as for the others.
+// Some systems refuse to page-lock memory that exists already: hipErrorNotSupported, or hipErrorInvalidValue for a range that is there.  The arrays then stay
+// pageable: dn_batch_upload asks every pointer what it is and waits for its copies.  The refused pointers are kept so that dn_host_unregister answers for them as
+// for the others.  Every other failure is the caller's to know.
 static std::mutex g_pageable_mu;
 static std::vector<void *> g_pageable;
+static bool host_mapped(const void *p, size_t bytes) {     // every page of the range belongs to the process
+    const uintptr_t page = (uintptr_t)sysconf(_SC_PAGESIZE), at = (uintptr_t)p & ~(page - 1), end = (uintptr_t)p + bytes;
+    if (end < (uintptr_t)p) return false;
+    unsigned char seen[4096];
+    for (uintptr_t a = at; a < end; a += sizeof seen * page)
+        if (mincore((void *)a, std::min<size_t>(end - a, sizeof seen * page), seen)) return false;
+    return true;
+}
 int dn_host_register(void *p, size_t bytes) {
     if (!p || !bytes) return DN_ERR_ARG;
-    if (hipHostRegister(p, bytes, hipHostRegisterDefault) == hipSuccess) return DN_OK;
-    (void)hipGetLastError();                               // the refusal must not surface after the next launch
+    const hipError_t e = hipHostRegister(p, bytes, hipHostRegisterDefault);
     std::lock_guard<std::mutex> lk(g_pageable_mu);
-    if (g_pageable.empty()) fprintf(stderr, "dnascent_hip: the system does not page-lock existing memory; uploads from it wait for their copies\n");
-    g_pageable.push_back(p);
+    if (e == hipSuccess) {                                 // (its address may be that of an array that was refused and freed without a word)
+        g_pageable.erase(std::remove(g_pageable.begin(), g_pageable.end(), p), g_pageable.end());
+        return DN_OK;
+    }
+    (void)hipGetLastError();                               // the refusal must not surface after the next launch
+    if ((e != hipErrorNotSupported && e != hipErrorInvalidValue) || !host_mapped(p, bytes)) return DN_ERR_HIP;
+    try { g_pageable.push_back(p); } catch (...) { return DN_ERR_HIP; }
+    if (g_pageable.size() == 1) fprintf(stderr, "dnascent_hip: the system does not page-lock existing memory; uploads from it wait for their copies\n");
     return DN_OK;
 }
 int dn_host_unregister(void *p) {

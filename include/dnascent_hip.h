@@ -89,7 +89,8 @@ typedef struct {
 int dn_batch_upload(dn_ctx *ctx, const dn_batch_desc *batch);
 /* page-locked host memory for the input arrays: hipHostMalloc / hipHostRegister behind a C signature.  Where the system refuses to
  * page-lock memory that exists already, dn_host_register still returns DN_OK: the memory stays pageable and uploads from it wait for
- * their copies (dn_batch_upload asks every pointer); memory that must be page-locked comes from dn_host_alloc. */
+ * their copies (dn_batch_upload asks every pointer); memory that must be page-locked comes from dn_host_alloc.  A range that is not the
+ * process's, one that is registered already, no device and no memory left are errors (DN_ERR_HIP). */
 int dn_host_alloc(size_t bytes, void **p);
 void dn_host_free(void *p);
 int dn_host_register(void *p, size_t bytes);
