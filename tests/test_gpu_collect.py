@@ -187,3 +187,44 @@ def test_reserve_sizes_the_workspace_once(model):
     small.upload(ref); ref.run("normalise"); ref.sync()
     assert got.tobytes() == ref.summaries().tobytes()
     ctx.close(); ref.close()
+
+
+def _page_locked(desc, reserve):
+    """the batch with every array copied into memory of dn_host_alloc, and that memory.  reserve: bytes in front of each array, to place it off its block's start"""
+    import ctypes as C
+    L = hip.lib()
+    n = int(desc.n_reads)
+    last = lambda p: int(C.cast(p, C.POINTER(C.c_uint64))[n])  # noqa: E731
+    adc, base, ref = last(desc.adc_off), last(desc.basecall_off), last(desc.refseq_off)
+    sizes = dict(adc=2 * adc, adc_off=8 * (n + 1), cal_offset=4 * n, cal_scale=4 * n, basecall=base, basecall_off=8 * (n + 1), refseq=ref, refseq_off=8 * (n + 1),
+                 ref2query=4 * ref, query2ref=4 * (base + n), ref2del=ref, ref_start=4 * n, ref_end=4 * n, is_reverse=n)
+    out, held = hip.BatchDesc(), []
+    out.n_reads = n
+    for name, size in sizes.items():
+        p = C.c_void_p()
+        assert L.dn_host_alloc(size + reserve, C.byref(p)) == 0
+        held.append(p)
+        C.memmove(p.value + reserve, getattr(desc, name), size)
+        setattr(out, name, p.value + reserve)
+    return out, held, sizes
+
+
+@pytest.mark.parametrize("reserve", [0, 64])
+def test_page_locked_memory_of_the_library_uploads_asynchronously(model, reserve):
+    """arrays of dn_host_alloc are page-locked wherever the library runs (arrays that exist already may stay pageable), so this upload returns before its copies
+    are done: the same bits through two contexts at once, and after the arrays have been overwritten behind dn_sync"""
+    import ctypes as C
+    b, reads = _batch(model, SPECS)
+    a = _ctx(model); b.upload(a); a.run("detect"); want = a.collect()
+    desc, held, sizes = _page_locked(b.desc(), reserve)
+    c, d = _ctx(model), _ctx(model)
+    for x in (c, d):
+        x.upload(desc, b.size(), keep=held); x.run("detect")
+    _same(want, c.collect()); _same(want, d.collect())
+    c.upload(desc, b.size(), keep=held); c.sync()
+    C.memset(desc.adc, 0, sizes["adc"])                    # the copies are done
+    c.run("detect"); _same(want, c.collect())
+    for x in (a, c, d):
+        x.close()
+    for p in held:
+        hip.lib().dn_host_free(p)
