@@ -184,7 +184,8 @@ def main():
     ap.add_argument("--reads-per-step", type=int, default=None, help="reads per batch (default 500 full / 1000 banded)")
     ap.add_argument("--bases", type=int, default=None, help="bases per read (default 50000 full / 20000 banded)")
     ap.add_argument("--inflight", type=int, default=None,
-                    help="batches in flight per GPU, each on its own context / stream / workspace (default 8)")
+                    help="batches in flight per GPU, each on its own context / stream / workspace (default: 6 through the network, 8 in the banded scope, fewer where "
+                         "the process has fewer than eight hardware queues)")
     ap.add_argument("--emit", type=int, default=1, help="full scope: format + write the .detect records inside the timed region")
     ap.add_argument("--out", default=None, help="full scope: .detect output path (default: formatted and counted, not written)")
     ap.add_argument("--cnn-math", choices=["f16x3", "bf16x6", "fp32"], default=None)
@@ -201,7 +202,9 @@ def main():
     bases = args.bases or (50000 if full else 20000)
     # contexts (batches) in flight.  Full pipeline, one session of round 5 (gpurun_out/r5w, --steps 14): 4 -> 808 / 805, 5 -> 813 / 813, 6 -> 821 / 822, 8 -> 816 / 814
     # Msamples/s; 6 x 14.5 GB of workspaces + 4 CNN lanes x 16 GiB = 159 of 309 GB (8: 189).  The banded scope (no network) keeps 8.
-    inflight = args.inflight or (6 if full else 8)
+    # (Eight hardware queues; with fewer, what hip.batches_in_flight says.)
+    from dnascent_amd import hip as _hip
+    inflight = args.inflight or _hip.batches_in_flight(6 if full else 8, network=full)
     os.environ.setdefault("DN_CNN_ROWS", str(8 << 20))      # activation rows resident per CNN pass and lane: 8 Mi rows = 32 GiB, three passes per 500 x 50 kb batch (round 5, with the persistent
     # whole-CU kernels in the network: 4 Mi 853-857, 6 Mi 862-863, 8 Mi 870-874 Msamples/s, profiles/r05_cnn_pass_rows_ab.txt; round 4: 2 Mi -6 %, 8 Mi -3 %)
 

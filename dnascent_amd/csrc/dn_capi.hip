@@ -433,8 +433,8 @@ int dn_ctx_create(int device, void *hip_stream, dn_ctx **out) {
     { std::lock_guard<std::mutex> lk(g_lane_mu); c->lane_id = (g_ctx_seq++) % lane_count(); if (device < 64) g_dev_ctx[device]++; }
     if (hip_stream) { c->stream = (hipStream_t)hip_stream; c->own_stream = false; }
     else {
-        // every stream has the default priority: per-batch streams above the CNN lanes' and below them measured the same (841-862 Msamples/s,
-        // two repetitions per setting)
+        // every stream has the default priority: work on streams of different priorities has hung for good on some machines.  What that costs: with the
+        // batches' streams above the CNN lanes' the default benchmark ran at 876 Msamples/s on eight hardware queues, without at 828-844
         bool made = false;
         if (front_cus()) {
             uint32_t m[8]; front_mask(m, false);

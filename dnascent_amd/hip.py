@@ -181,6 +181,23 @@ class DnError(RuntimeError):
     pass
 
 
+def batches_in_flight(most, network=True):
+    """How many batches (contexts) to keep in flight on a device: `most`, or what the process's hardware queues carry.
+
+    Every context has a stream and, with the network, uses one of the device's CNN lanes; streams that share a hardware queue wait for each other, and a batch whose
+    short launches stand behind another one's network loses more than another batch in flight gains.  Msamples/s, 500 x 50 kb batches through the network --
+    4 queues: 3 in flight 821-828, 4 685, 5 733, 6 639; 6 queues: 3 816, 4 831, 6 710; 8 queues: 3 834, 4 844, 6 828-838.  1-200 kb reads -- 4 queues: 3 617, 5 548;
+    8 queues: 3 612, 5 712.  Without the network (1000 x 20 kb) -- 4 queues: 3 11141, 4 11785, 8 10047; 8 queues: 8 13099.
+    The number of queues is GPU_MAX_HW_QUEUES, as it was when the HIP runtime started; 8, what the library asks for, if it is not set."""
+    try:
+        queues = int(os.environ.get("GPU_MAX_HW_QUEUES", "8"))
+    except ValueError:
+        queues = 4                                         # ROCm's own default
+    if queues >= 8:
+        return most
+    return min(most, max(3, queues // 2 + 1) if network else max(1, queues))
+
+
 _dense8_module = None
 
 

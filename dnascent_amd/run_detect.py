@@ -80,7 +80,8 @@ def main(argv=None):
     ap.add_argument("--out", required=True)
     ap.add_argument("--model", default=None, help="CNN description prefix (tools/convert_savedmodel.py); default: synthetic weights")
     ap.add_argument("--pore-model", default=None)
-    ap.add_argument("--inflight", type=int, default=5, help="batches in flight on the GPU (one context each: ~14.5 GB of HBM per 300 M samples at the default event bound).  "
+    ap.add_argument("--inflight", type=int, default=None, help="batches in flight on the GPU (one context each: ~14.5 GB of HBM per 300 M samples at the default event bound).  "
+                    "Default 5, fewer where the process has fewer than eight hardware queues (hip.batches_in_flight).  With eight, "
                     "4-8 stream alike (bench.py: within 1.5 %%); from 6 up the contexts' 160+ GB of hipMalloc, which run beside the first batches, took 3.5 s instead of 1 "
                     "in most runs (gpurun_out/r5v: 10 000 x 50 kb in 7.8-7.9 s at 4 and 5, 10.0-10.6 s at 6, 7.9-10.0 s at 8)")
     ap.add_argument("--batch-samples", type=float, default=300e6, help="sample budget of one batch")
@@ -118,6 +119,8 @@ def main(argv=None):
         dist.barrier(device_ids=[int(dev_t.split(":")[1])]) if dev_t != "cpu" else dist.barrier()
 
     from dnascent_amd import cnn_model, hip, host, shard, synth
+    if a.inflight is None:
+        a.inflight = hip.batches_in_flight(5)
     t0 = time.time()
     sizes, offsets = host.container_index(a.container)
     t_index = time.time() - t0
