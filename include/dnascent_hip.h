@@ -278,8 +278,9 @@ int dn_debug_emission(dn_ctx *ctx, uint32_t n, const double *x, const double *mu
  * Unlike the stages above these calls work on the CALLER's device memory (plain pointers of the context's device, rows at a pitch of ld elements),
  * are enqueued on the caller's stream (hip_stream: a hipStream_t, NULL = the default stream) and keep nothing: no allocation, no
  * synchronisation, no state in the context but the error text, so they can be captured into a graph and run on several streams at once.
- * The workspace belongs to the caller (dn_i8_*_workspace bytes, 256-byte aligned; those two calls look at the description only, ctx may be NULL) and must
- * not be shared by calls that can overlap.  Outputs must not
+ * The workspace belongs to the caller (dn_i8_*_workspace bytes, 256-byte aligned) and must not be shared by calls that can overlap.  Those two calls look at the
+ * description only (ctx may be NULL), at all of it: sizes, types, which results are asked for, and the addresses and pitches of x, q and w, of which only multiples of
+ * 16 bytes are read in place.  Ask with the description of the call.  Outputs must not
  * overlap inputs or each other.  M may be 0; 1 <= N, K <= DN_I8_MAX_K; 0 <= M < DN_I8_MAX_M.  Rows at a multiple of 16 bytes
  * (what dn_i8_rows' callers are advised to choose) are read directly, others through the workspace. */
 enum { DN_T_F32 = 0, DN_T_F16 = 1, DN_T_BF16 = 2, DN_T_I8 = 3 };

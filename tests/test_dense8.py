@@ -68,6 +68,17 @@ def test_grad_refuses(kw):
     assert _ask("dn_i8_linear_grad", _grad(**kw))[0] == -3
 
 
+@pytest.mark.parametrize("kw,rows", [(dict(ldw=297), 0), (dict(w=P + 1), 0), (dict(x=P + 8), 1), (dict(ldx=297), 1)])
+def test_workspace_follows_addresses_and_pitches(kw, rows):
+    """rows that do not lie at multiples of 16 bytes are copied to where they do (rows of more than 256 codes; narrower ones are read
+    as they lie): 304 bytes for 297 codes, w's 300 rows or x's 200"""
+    wide = dict(m=200, n=300, k=297, x=P, ldx=304, x_type=3, sx=P, ldw=304, ldy=300)
+    rc, base = _ask("dn_i8_linear", _linear(**wide))
+    wide.update(kw)
+    rc2, need = _ask("dn_i8_linear", _linear(**wide))
+    assert rc == rc2 == 0 and need - base == -(-(200 if rows else 300) * 304 // 256) * 256
+
+
 def test_null_arguments():
     L = hip.lib()
     n = C.c_uint64(0)

@@ -846,3 +846,28 @@ def _border(got, want, terms, u):
     room = half * want.abs() + u * terms
     near = (want.abs() - room <= top) & (want.abs() + room >= top * (1 + half)) & (got == want.sign() * math.inf)
     return torch.where(near, (want.sign() * top).to(got.dtype), got)
+
+
+def test_a_workspace_of_another_description_is_refused(ctx):
+    """the size for rows at multiples of 16 bytes does not do for the same shape elsewhere; the size for the call itself does"""
+    L = hip.lib()
+    m, n, k = 200, 300, 297
+    x = some_rows(m, k, BF16, 71)
+    q, s = ctx.i8_rows(x)
+    wq, ws = eight(n, k, 72)
+    odd = torch.zeros(n * k + 1, dtype=torch.int8, device="cuda")[1:].view(n, k)
+    odd.copy_(wq)
+    y = torch.empty(m, n, dtype=BF16, device="cuda")
+
+    def desc(w):
+        return hip.i8_desc(hip.I8_LINEAR_FIELDS, m=m, n=n, k=k, x=q.data_ptr(), ldx=q.stride(0), sx=s.data_ptr(), w=w.data_ptr(), ldw=w.stride(0), sw=ws.data_ptr(),
+                           y=y.data_ptr(), ldy=n, x_type=3, y_type=2)
+    need = [C.c_uint64(0), C.c_uint64(0)]
+    for w, v in zip((wq, odd), need):
+        assert L.dn_i8_linear_workspace(ctx.h, desc(w), C.byref(v)) == 0
+    assert need[1].value > need[0].value
+    space = torch.empty(need[1].value, dtype=torch.uint8, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    assert L.dn_i8_linear(ctx.h, desc(odd), space.data_ptr(), need[0].value, st) == -3 and b"workspace" in L.dn_last_error(ctx.h)
+    assert L.dn_i8_linear(ctx.h, desc(odd), space.data_ptr(), need[1].value, st) == 0
+    assert torch.equal(y, ctx.i8_linear(q, wq, ws, sx=s))
