@@ -96,6 +96,14 @@ def _run(ctx, entry, desc):
         ctx._chk(rc, entry)
 
 
+def _no_gradient(**tensors):
+    """the calls give tensors without a history: one that asks for a gradient would lose it without a word"""
+    if torch.is_grad_enabled():
+        for name, t in tensors.items():
+            if t is not None and t.requires_grad:
+                raise ValueError("%s requires a gradient, which this call does not pass on: use dense8.Dense, torch.no_grad() or .detach()" % name)
+
+
 def rows(ctx, x):
     _check(ctx, "x", x, _NUMBERS)
     m, k, ldx = _rows("x", x)
@@ -113,6 +121,7 @@ def restore(ctx, q, s, dtype):
         raise TypeError("dtype is %s" % dtype)
     m, k, ldq = _rows("q", q)
     at = _vector(ctx, "s", s, q.shape[:-1])
+    _no_gradient(s=s)
     x = torch.empty(q.shape, dtype=dtype, device=q.device)
     rc = hip.lib().dn_i8_restore(ctx.h, m, k, q.data_ptr(), ldq, at, x.data_ptr(), k, TYPES[dtype], _stream(ctx.device))
     if rc:
@@ -138,6 +147,7 @@ def linear(ctx, x, wq, ws, sx=None, bias=None, residual=None, relu=False, out_dt
     out_dtype = out_dtype or (torch.bfloat16 if given else x.dtype)
     if out_dtype not in _NUMBERS:
         raise TypeError("out_dtype is %s" % out_dtype)
+    _no_gradient(x=x, ws=ws, sx=sx, bias=bias, residual=residual)
     lead = x.shape[:-1]
     at_sx = _vector(ctx, "sx", sx, lead) if given else 0
     at_bias = _vector(ctx, "bias", bias, (n,)) if bias is not None else 0
@@ -178,6 +188,7 @@ def linear_grad(ctx, dy, q, s, wq, ws, mask=None, need_dx=True, need_dw=True, ne
     nw, ldw, at_ws = _weight(ctx, wq, ws, k)
     if nw != n:
         raise ValueError("wq has %d output channels, dy %d" % (nw, n))
+    _no_gradient(dy=dy, s=s, ws=ws)
     w_dtype = w_dtype or dy.dtype
     if w_dtype not in _NUMBERS:
         raise TypeError("w_dtype is %s" % w_dtype)

@@ -427,7 +427,7 @@ class Context:
     def i8_rows(self, x):
         """dn_i8_rows: x [..., K] (fp32, fp16 or bf16) as rows of 8-bit integers and one fp32 scale each -> (q [..., K] int8, s [...]).  A row of q
         starts at a multiple of 16 bytes (its pitch is K rounded up), which is how i8_linear and i8_linear_grad read rows fastest; a weight [N, K]
-        becomes (wq, ws) the same way, once."""
+        becomes (wq, ws) the same way, once.  The result has no gradient history."""
         return _dense8().rows(self, x)
 
     def i8_restore(self, q, s, dtype):
@@ -437,12 +437,13 @@ class Context:
     def i8_linear(self, x, wq, ws, sx=None, bias=None, residual=None, relu=False, out_dtype=None, save=False):
         """dn_i8_linear: y [..., N] = act(x W^T + bias + residual) with x [..., K] in 8 bits: numbers (then their rows are made on the way), or int8 rows
         with their scales sx.  wq [N, K] int8, ws [N] fp32, bias [N] fp32, residual [..., N] of y's type.  out_dtype: x's type, or bf16 for int8 rows.
-        save=True: (y, dense8.Saved) -- what i8_linear_grad needs: the rows, their scales and, with relu, one bit per output."""
+        save=True: (y, dense8.Saved) -- what i8_linear_grad needs: the rows, their scales and, with relu, one bit per output.
+        The result has no gradient history: an argument that requires a gradient is refused outside torch.no_grad() (dense8.Dense is the layer that has one)."""
         return _dense8().linear(self, x, wq, ws, sx, bias, residual, relu, out_dtype, save)
 
     def i8_linear_grad(self, dy, q, s, wq, ws, mask=None, need_dx=True, need_dw=True, need_db=True, w_dtype=None):
         """dn_i8_linear_grad: (dx [..., K] of dy's type, dw [N, K], db [N], both of w_dtype: dy's type if not given) for dy [..., N] from the 8-bit rows
-        of the layer's input; None for what is not needed.  mask: dense8.Saved.mask of a layer with a ReLU."""
+        of the layer's input; None for what is not needed.  mask: dense8.Saved.mask of a layer with a ReLU.  The results have no gradient history, as i8_linear's."""
         return _dense8().linear_grad(self, dy, q, s, wq, ws, mask, need_dx, need_dw, need_db, w_dtype)
 
     # ---- measurement ------------------------------------------------------------------------

@@ -133,3 +133,16 @@ def test_tensors_of_another_device_are_refused():
             call()
     with pytest.raises(TypeError):
         dense8.rows(ctx, x.numpy())
+
+
+def test_arguments_that_require_a_gradient_are_refused():
+    """i8_linear, i8_linear_grad and i8_restore give tensors without a history; on tensors of no device, which the checks in front of the first call see"""
+    ctx = SimpleNamespace(device=-1, h=None)
+    x, q, s, b = torch.zeros(2, 8), torch.zeros(3, 8, dtype=torch.int8), torch.zeros(3), torch.zeros(3)
+    x8, sx, r = torch.zeros(2, 8, dtype=torch.int8), torch.zeros(2), torch.zeros(2, 3)
+    grad = lambda t: t.clone().requires_grad_()  # noqa: E731
+    for name, call in [("x", lambda: dense8.linear(ctx, grad(x), q, s)), ("ws", lambda: dense8.linear(ctx, x, q, grad(s))), ("bias", lambda: dense8.linear(ctx, x, q, s, bias=grad(b))),
+                       ("residual", lambda: dense8.linear(ctx, x, q, s, residual=grad(r))), ("sx", lambda: dense8.linear(ctx, x8, q, s, sx=grad(sx))),
+                       ("s", lambda: dense8.restore(ctx, q, grad(s), torch.float32)), ("dy", lambda: dense8.linear_grad(ctx, grad(r), x8, sx, q, s))]:
+        with pytest.raises(ValueError, match="^%s requires a gradient" % name):
+            call()

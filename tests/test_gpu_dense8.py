@@ -871,3 +871,16 @@ def test_a_workspace_of_another_description_is_refused(ctx):
     assert L.dn_i8_linear(ctx.h, desc(odd), space.data_ptr(), need[0].value, st) == -3 and b"workspace" in L.dn_last_error(ctx.h)
     assert L.dn_i8_linear(ctx.h, desc(odd), space.data_ptr(), need[1].value, st) == 0
     assert torch.equal(y, ctx.i8_linear(q, wq, ws, sx=s))
+
+
+def test_calls_without_a_history(ctx):
+    """a tensor that requires a gradient: refused, but taken under no_grad and detached; i8_rows makes a parameter's rows"""
+    wq, ws = eight(24, 40, 81)
+    x = some_rows(30, 40, BF16, 82).requires_grad_()
+    with pytest.raises(ValueError, match="requires a gradient"):
+        ctx.i8_linear(x, wq, ws)
+    y = ctx.i8_linear(x.detach(), wq, ws)
+    with torch.no_grad():
+        assert torch.equal(ctx.i8_linear(x, wq, ws), y)
+    q, s = ctx.i8_rows(x)
+    assert not s.requires_grad and torch.equal(q, ctx.i8_rows(x.detach())[0])
