@@ -222,15 +222,19 @@ def _packed(t):
         return t.contiguous()
 
 
+def _dense(ctx, x, weight, bias, residual, relu, save):
+    """the layer's product: (what linear returns, the weight's rows, their scales)"""
+    wq, ws = rows(ctx, _packed(weight))
+    return linear(ctx, _packed(x), wq, ws, bias=None if bias is None else bias.float(), residual=None if residual is None else _packed(residual), relu=relu, save=save), wq, ws
+
+
 class _Layer(torch.autograd.Function):
     """The forward pass keeps what i8_linear saves and the weight's 8-bit rows; both quantisers count as the identity in the backward pass, so the gradients
     are those of the product that was computed."""
 
     @staticmethod
     def forward(fn, x, weight, bias, residual, ctx, relu):
-        wq, ws = rows(ctx, _packed(weight))
-        b = None if bias is None else bias.float()
-        y, saved = linear(ctx, _packed(x), wq, ws, bias=b, residual=None if residual is None else _packed(residual), relu=relu, save=True)
+        (y, saved), wq, ws = _dense(ctx, x, weight, bias, residual, relu, True)
         fn.save_for_backward(saved.q, saved.s, saved.mask, wq, ws)
         fn.ctx, fn.w_dtype, fn.b_dtype = ctx, weight.dtype, None if bias is None else bias.dtype
         return y
@@ -253,7 +257,7 @@ class _Layer(torch.autograd.Function):
 
 class Dense(torch.nn.Module):
     """y [..., N] = act(x W^T + b (+ residual)) whose forward pass multiplies 8-bit rows and whose backward pass reads them again: weight [N, K] and bias [N] are
-    parameters (fp32, fp16 or bf16) on ctx's device; x [..., K] of the same types.  Between the passes a row of x costs K + 4 bytes.
+    parameters (fp32, fp16 or bf16) on ctx's device; x [..., K] of the same types.  Between the passes a row of x costs K + 4 bytes, without gradients nothing.
 
     A pass can be captured into a graph like any of torch's (its workspaces are torch tensors); as with those, no eager graph over the same parameters
     may be alive while a backward pass is being captured.
@@ -278,6 +282,8 @@ class Dense(torch.nn.Module):
         return new
 
     def forward(self, x, residual=None):
+        if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.weight, self.bias, residual))):
+            return _dense(self.ctx, x, self.weight, self.bias, residual, self.relu, False)[0]           # nothing to keep
         return _Layer.apply(x, self.weight, self.bias, residual, self.ctx, self.relu)
 
     @staticmethod

@@ -884,3 +884,25 @@ def test_calls_without_a_history(ctx):
         assert torch.equal(ctx.i8_linear(x, wq, ws), y)
     q, s = ctx.i8_rows(x)
     assert not s.requires_grad and torch.equal(q, ctx.i8_rows(x.detach())[0])
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 24, 40), (700, 256, 256), (2000, 300, 520)])
+def test_layer_without_gradients_keeps_nothing(ctx, m, n, k, monkeypatch):
+    from dnascent_amd import dense8
+    layer = dense8.Dense(ctx, k, n, relu=True)
+    x, res = some_rows(m, k, BF16, 91), some_rows(m, n, BF16, 92)
+    want = layer(x, res)
+    assert want.requires_grad
+    kept = []
+    plain = dense8.linear
+    monkeypatch.setattr(dense8, "linear", lambda *a, **kw: kept.append(kw.get("save", False)) or plain(*a, **kw))
+    with torch.no_grad():
+        y = layer(x.clone().requires_grad_(), res)
+    assert torch.equal(y, want.detach()) and not y.requires_grad
+    for p in layer.parameters():
+        p.requires_grad_(False)
+    y = layer(x, res)                                      # gradients are on, and nothing asks for one
+    assert torch.equal(y, want.detach()) and not y.requires_grad
+    assert kept == [False, False]
+    layer.bias.requires_grad_(True)
+    assert layer(x, res).requires_grad and kept[-1]
