@@ -103,8 +103,9 @@ __device__ __forceinline__ K8Pow k8_pow(unsigned top) {
 // ---- dx, narrow layers (N <= 256) ------------------------------------------------------------------------------------------------------------------------------
 // The same shape as the forward pass over narrow rows (k8_narrow): a wavefront takes 16 rows of dy, holds them in registers in the matrix operand's order, finds
 // each row's power of two, and multiplies with the weight, whose transposed fragments lie in LDS as fp16 (256 k x N).  Nothing but dy, the mask and dx moves.
-// NP: pieces.  512 threads keep everything in registers; 768 hide more but spill (100000 x 256 x 256 with dw, bf16, us: 80 : 91; 1 Mi rows, 499 : 517).
-// 1 Mi x 256 x 256 bf16 with ReLU: 252 us; its 1.1 GB take 213 at a copy's rate, its products 104, and the vector instructions that mask, scale and convert about as long.
+// NP: pieces.  512 threads, so that a lane has 256 registers: enough up to N = 128, and for N = 256 all but 9 (bf16), 15 (fp16) or 58 (fp32), which go to memory; 768 threads
+// hide more but keep less (100000 x 256 x 256 with dw, bf16, us: 80 : 91; 1 Mi rows, 499 : 517).
+// 1 Mi x 256 x 256 bf16 with ReLU: 260 us; its 1.1 GB take 213 at a copy's rate, its products 104, and the vector instructions that mask, scale and convert about as long.
 template <class T, int NS, int NP>
 __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d, uint8_t *__restrict__ again) {
     constexpr int WG = 512;
@@ -1312,7 +1313,8 @@ Plan plan_grad(const dn_i8_grad_desc &d) {
     // dw's tiles and the runs of rows: what costs least, by times measured on whole chips -- a workgroup's row in a tile of 256: 55 ns (fp16, fp32: 65), of 128: 21; its start and
     // end: 14 us and 9; a run's results, written and read again: 1.2 ps each.  bf16, us, 256 : 128 -- 1048576 x 256 x 256, 281 : 345; 200000 x 192 x 192, 73 : 89;
     // 50000 x 1024 x 256, 103 : 85; 7552 x 1664 x 1216, 82 : 139; 1000 x 1024 x 1024, 39 : 23; 64 x 2048 x 4096, 20 : 26;
-    // with dx, fp16, 12824 x 1088 x 2304, 310 : 338; fp32, 100000 x 256 x 256, 131 : 116
+    // with dx, fp16, 12824 x 1088 x 2304, 310 : 338; fp32, 100000 x 256 x 256, 131 : 116.  (Of a lane's 256 registers tiles of 256 lack 5 for bf16 and 7 for fp16; for fp32 17,
+    // or 80 with fp32 results: those go to memory.)
     if (std::max(d.n, d.k) <= 64) p.s = 64;
     else {
         double least = 1e30;

@@ -906,3 +906,19 @@ def test_layer_without_gradients_keeps_nothing(ctx, m, n, k, monkeypatch):
     assert kept == [False, False]
     layer.bias.requires_grad_(True)
     assert layer(x, res).requires_grad and kept[-1]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("m,n,k", [(9, 60, 40), (16, 300, 90), (200, 64, 64), (300, 128, 100), (20000, 250, 70), (400, 700, 130)])
+def test_grad_with_channel_scales_far_apart_and_zero(ctx, m, n, k, relu, dtype):
+    """output channels whose weights are 2^-30 to 2^6 of each other, some of them nothing at all (a dead channel), and a layer of dead channels only"""
+    dy, q, s, wq, ws, mask = grad_case(m, n, k, dtype, 7 * m + n, relu)
+    ws = ws * torch.exp2(torch.randint(-30, 7, (n,), generator=gen(n), device="cuda").float())
+    ws[::5] = 0
+    ws[n // 2] = 2.0 ** 10
+    got, ref = ctx.i8_linear_grad(dy, q, s, wq, ws, mask=mask), grad_ref(dy, q, s, wq, ws, mask)
+    check_grad(got, ref, m, n, dtype, dtype)
+    dead = torch.zeros_like(ws)
+    dx, dw, db = ctx.i8_linear_grad(dy, q, s, wq, dead, mask=mask)
+    assert not dx.any() and torch.equal(dw, got[1]) and torch.equal(db, got[2])
