@@ -17,7 +17,6 @@ HIP_SO = os.path.join(LIB, "libdnascent_hip.so")
 HOST_SO = os.path.join(LIB, "libdnascent_host.so")
 
 HIP_SOURCES = ["dn_capi.hip", "k1_segment.hip", "k2_banded.hip", "k_scaling.hip", "k2b_viterbi.hip", "k3_cnn.hip", "k_hmm.hip", "k_collect.hip", "k8_dense.hip", "k8_grad.hip"]
-PACKED_FP32 = {"k3_cnn.hip"}                              # writes packed fp32 instructions by hand; everywhere else the compiler makes none
 HOST_SOURCES = ["host/dn_synth.c", "host/dn_host.cpp", "host/dn_bam.cpp", "host/dn_vbz.cpp"]       # dn_bam.cpp: BGZF / BAM over zlib (libz is in the image; htslib is not); dn_vbz.cpp: POD5's signal codec (zstd through dlopen)
 
 
@@ -52,12 +51,13 @@ def build_hip(force=False):
     flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
              "-fno-fast-math", "-Wall", "-Wno-unused-function", "-Wno-unused-value", "-Wno-unused-result",
              "-fhip-fp32-correctly-rounded-divide-sqrt",
+             # no packed fp32 instructions: some of their forms have given wrong results on this hardware now and then
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
              "-I", os.path.join(ROOT, "include"), "-I", CSRC] + os.environ.get("DN_HIPCC_FLAGS", "").split()   # DN_HIPCC_FLAGS: experiment builds (-DDN_WS_TRACE=<workgroup>)
     objs, jobs = [], []
     for s in srcs:
         o = os.path.join(LIB, os.path.basename(s) + ".o")
-        unpacked = [] if os.path.basename(s) in PACKED_FP32 else ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-        jobs.append([hipcc] + flags + unpacked + ["-c", s, "-o", o])
+        jobs.append([hipcc] + flags + ["-c", s, "-o", o])
         objs.append(o)
     with ThreadPoolExecutor(min(len(jobs), int(os.environ.get("MAX_JOBS", "6")))) as pool:
         list(pool.map(_run, jobs))

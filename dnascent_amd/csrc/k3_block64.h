@@ -146,7 +146,7 @@ __device__ __forceinline__ void b64_split_store(const b64f2 (&o)[8], float &am, 
 }
 
 // a stage's epilogue: folded BatchNorm, ReLU, padding mask (MASKED: some row of the chunk is padding); accumulator register q of lane (n, hh) is row
-// (q & 3) + 8 (q >> 2) + 4 hh, column tile j is channel 2 n + j.  Rows go in pairs (q, q + 1): adjacent registers for the packed FMA.
+// (q & 3) + 8 (q >> 2) + 4 hh, column tile j is channel 2 n + j.  Rows go in pairs (q, q + 1).
 template <bool MASKED, bool TO_GLOBAL>
 __device__ __forceinline__ void b64_epilogue(const f32x16 (&acc)[2], const b64f2 sc, const b64f2 sh, const float floor_, const unsigned vml, float *wrow,
                                              const __amdgpu_buffer_rsrc_t rY, const int ybase) {
@@ -276,7 +276,7 @@ __device__ __forceinline__ void b64_stage(const B64Args &A, const int st, const 
                     }
                 }
                 B64_T(st, 1 + 4 * cb);
-                // ---- depthwise: output row 8 rq + i = sum over taps t of in[8 rq + i + t] w[t], taps ascending (k3_dwconv's order), packed over the channel pair ----
+                // ---- depthwise: output row 8 rq + i = sum over taps t of in[8 rq + i + t] w[t], taps ascending (k3_dwconv's order), a channel pair at a time ----
                 b64f2 o[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) o[i] = b64f2{0.f, 0.f};
@@ -285,7 +285,7 @@ __device__ __forceinline__ void b64_stage(const B64Args &A, const int st, const 
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int t = j - i;
-                        if (t >= 0 && t < 5) asm volatile("v_pk_fma_f32 %0, %1, %2, %0" : "+v"(o[i]) : "v"(x[j]), "v"(tw[cb][t]));
+                        if (t >= 0 && t < 5) k3_fma2(o[i], x[j], tw[cb][t]);
                     }
                 }
                 B64_T(st, 2 + 4 * cb);
@@ -460,7 +460,7 @@ __device__ __forceinline__ void b64_conv(const B64Args &A, const int ct, const i
 // layer l's sums ALSO filters them for layer l + 1, in the registers they are already in: after the epilogue lane (n, hh) holds channels (2 n, 2 n + 1) of
 // rows {0-3, 8-11, 16-19, 24-27} + 4 hh -- a 5-tap filter down the rows needs its neighbours' rows, and four rounds of v_permlane32_swap (the lane halves
 // exchange register halves; no LDS) turn that into 20 CONSECUTIVE rows per lane: rows -4 .. 15 in the lower half, 12 .. 31 in the upper, the first four of
-// the lower half being the chunk before's last four, which the wavefront keeps in registers.  Each half then filters 16 output rows (80 packed FMAs, taps
+// the lower half being the chunk before's last four, which the wavefront keeps in registers.  Each half then filters 16 output rows (80 pairs of FMAs, taps
 // ascending as everywhere), splits them and stores layer l + 1's fp16 planes.  LDS per layer boundary: ONE crossing (planes written, planes read) instead of
 // two, 40 instructions instead of ~72; the fp32 rings and the halo rows are gone (only the last layer still hands fp32 rows to the shortcut's join).
 //
@@ -607,7 +607,7 @@ __device__ __forceinline__ void b64_v3_stage(const B64Args &A, const int st, con
 #pragma unroll
                 for (int k = 0; k < 16; k++) {
                     const int t = w - k;
-                    if (t >= 0 && t < 5) asm volatile("v_pk_fma_f32 %0, %1, %2, %0" : "+v"(o[k >> 3][k & 7]) : "v"(W[w]), "v"(tw[t]));
+                    if (t >= 0 && t < 5) k3_fma2(o[k >> 3][k & 7], W[w], tw[t]);
                 }
             }
             B64_T(st, 4);
@@ -677,7 +677,7 @@ __device__ __forceinline__ void b64_v3_ends(const B64Args &A, const int lane, co
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int t = j - i;
-                        if (t >= 0 && t < 5) asm volatile("v_pk_fma_f32 %0, %1, %2, %0" : "+v"(o[i]) : "v"(x[j]), "v"(tw[cb][t]));
+                        if (t >= 0 && t < 5) k3_fma2(o[i], x[j], tw[cb][t]);
                     }
                 }
                 gloadX(s + 1, cb);                          // (past the stripe: loaded, never used)

@@ -73,14 +73,22 @@ template <int CHUNK> __device__ __forceinline__ void gru_wload(WChunk &w, cfptr_
 }
 __device__ __forceinline__ void gru_wwait(WChunk &w) { asm volatile("s_waitcnt lgkmcnt(0)" : "+s"(w.a), "+s"(w.b)); }
 typedef float gf32x2 __attribute__((ext_vector_type(2)));
+// o += x w for a pair of channels, in the order in which the statements stand: volatile asm statements keep it.  (Two FMAs, not a packed one: some packed fp32 forms
+// have given wrong results on this hardware now and then.  Alone, ms, two : packed -- k3_block64 3.00 : 2.88, k3_pair128 2.70 : 2.57, k3_sep_ws 4.27 : 4.29; default benchmark,
+// 4 hardware queues 818-823 : 826-832 Msamples/s, 8 queues 839-844 : 834-845.)
+__device__ __forceinline__ void k3_fma2(gf32x2 &o, gf32x2 x, gf32x2 w) {
+    float a = o[0], b = o[1];
+    asm volatile("v_fmac_f32 %0, %2, %4\n\tv_fmac_f32 %1, %3, %5" : "+&v"(a), "+&v"(b) : "v"(x[0]), "v"(x[1]), "v"(w[0]), "v"(w[1]));
+    o = gf32x2{ a, b };
+}
 // the 32 weights of a chunk are 16 adjacent (output v, v + 1) pairs of ONE input j or of two consecutive ones (48 outputs per input):
-// v_pk_fma_f32 with the SGPR pair as one operand and h[j] broadcast to both halves -- half the vector instructions of v_fmac_f32
+// one FMA each, with the weight as its scalar operand
 template <int CHUNK> __device__ __forceinline__ void gru_wfma(const WChunk &w, const gf32x2 (&hh)[16], gf32x2 (&acc)[24]) {
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
         const int idx = CHUNK * 32 + e, j = idx / 48, v = idx % 48;          // weights W[j][v], W[j][v + 1]: input j, outputs v, v + 1 (z 0-15, r 16-31, g 32-47)
         const gf32x2 wv = e < 16 ? gf32x2{w.a[e], w.a[e + 1]} : gf32x2{w.b[e - 16], w.b[e - 15]};
-        asm("v_pk_fma_f32 %0, %1, %2, %0" : "+v"(acc[v / 2]) : "s"(wv), "v"(hh[j]));
+        acc[v / 2] = gf32x2{ __builtin_fmaf(wv[0], hh[j][0], acc[v / 2][0]), __builtin_fmaf(wv[1], hh[j][1], acc[v / 2][1]) };
     }
 }
 template <int C> struct GruSteps {
@@ -178,7 +186,7 @@ __global__ __launch_bounds__(64) void k3_encode(const float *core, const float *
 
 // ---------------------------------------------------------------------------------------------------------
 // k3_encode_mfma (round 3): the same encoder with the GRU's matrix-vector products on the MATRIX cores.  k3_encode spends ~2 200 vector
-// instructions per time step on three 16 x 48 products per position (wave-uniform weights as SGPR operands of v_pk_fma_f32); batched
+// instructions per time step on three 16 x 48 products per position (wave-uniform weights as scalar operands); batched
 // over the 32 positions of a wavefront they are 32 x 16 x 48 GEMMs -- v_mfma_f32_32x32x16_f16 with K = the 16 units exactly:
 //     D'[output (32 rows)][position (32 columns)] += W^T[output][unit] * h^T[unit][position]
 //   A operand = W^T: lane (i = lane & 31, hh = lane >> 5) holds the 8 inputs k' = 8 hh .. 8 hh + 7 of output row i
@@ -507,7 +515,7 @@ __device__ __forceinline__ void conv_epilogue(f32x16 (&acc)[2][BN / 64], float *
                 for (int j = 0; j < NJ; j++) addv[q][j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(ra, voff + j * 128, soff, 0));
             }
         }
-        // rows in pairs (q, q + 1): packed FMA and packed add; the padding select only where the wavefront's rows have padding at all
+        // rows in pairs (q, q + 1); the padding select only where the wavefront's rows have padding at all
         // (a tile in 140 on the 20 kb workload)
         typedef float f32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
@@ -659,7 +667,7 @@ __device__ __forceinline__ void split3(const f32x4 lo4, const f32x4 hi4, bf16x8 
     }
 }
 // One channel PAIR split into its two fp16 pieces (+ the range report's running maximum), the way every f16x3 kernel below does it.  K3_SPLIT_MIX:
-//   0  element by element as first written: per pair v_cvt_pk_f16_f32, 2 x v_cvt_f32_f16, v_pk_add_f32 (or 2 x v_sub_f32), v_cvt_pk_f16_f32, and 2-3 v_max_f32
+//   0  element by element as first written: per pair v_cvt_pk_f16_f32, 2 x v_cvt_f32_f16, 2 x v_sub_f32, v_cvt_pk_f16_f32, and 2-3 v_max_f32
 //      for the maximum (fmaxf (amax, fabsf (x)) per element: the compiler quiets a possible NaN of every operand first);
 //   2  the maximum as ONE v_max3_f32 (amax, |x0|, |x1|) per pair;
 //   1  that, and the rest x - (float) h as ONE v_fma_mix_f32 per element, which reads the fp16 half in place (h x -1.0 + x: exact, the same value).
@@ -1298,8 +1306,8 @@ __global__ __launch_bounds__(512) void k3_sep_ws(const float *__restrict__ X, fl
     // Depthwise filter of one producer wavefront: 32 output rows x 32 channels per channel block.  A lane owns a PAIR of adjacent
     // channels and 8 consecutive output rows: its 24 input rows and its 17 taps are each read ONCE from LDS as 8-byte pairs
     // (ds_read_b64; the first version re-read every input row 5 times and the taps per 4-row strip as 16-byte quads: 37 KB of LDS
-    // reads per wavefront and channel block, now 21 KB) and the filter runs as packed fp32 FMAs (v_pk_fma_f32: the two channels of
-    // the pair in one instruction, half the vector instructions), taps in ascending order -- bit-identical to k3_dwconv.
+    // reads per wavefront and channel block, now 21 KB) and the filter runs as two FMAs per pair
+    // (k3_fma2), taps in ascending order -- bit-identical to k3_dwconv.
     // Raw-slice pitch 36 floats: the two 16-lane row groups of a 32-lane LDS pass start 8 rows = 1152 B = half a bank window apart.
     auto depthwise = [&](int abuf, int wbuf) {
         typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -1310,8 +1318,8 @@ __global__ __launch_bounds__(512) void k3_sep_ws(const float *__restrict__ X, fl
         for (int i = 0; i < 8; i++) o[i] = f32x2{0.f, 0.f};
         // All input rows first, then per input row one GROUP of up to 8 independent FMAs (one per output row it meets), in exactly
         // this order: the FMAs are volatile asm statements, which keep their relative order.  Left to the compiler this became 8
-        // serial chains of 17 dependent v_pk_fma_f32 with a hazard nop after each (a dependent vector instruction issues every
-        // ~8.5 ticks, an independent one every ~5.5: tools/ubench_coissue.hip, profiles/r01_valu_issue_microbench.txt);
+        // serial chains of 17 dependent FMAs (a dependent vector instruction issues every ~8.5 ticks, an independent one every
+        // ~5.5: tools/ubench_coissue.hip, profiles/r01_valu_issue_microbench.txt);
         // __builtin_amdgcn_sched_barrier between the groups did not help, the chains are formed before the scheduler sees them.
         // The phase trace (tools/ws_trace.py) shows the producers' filter, not the matrix work, setting the pace of the workgroup.
         f32x2 x[KW + 7];
@@ -1322,7 +1330,7 @@ __global__ __launch_bounds__(512) void k3_sep_ws(const float *__restrict__ X, fl
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int t = j - i;                       // tap of output row dr + i that input row dr + j meets (ascending per output)
-                if (t >= 0 && t < KW) asm volatile("v_pk_fma_f32 %0, %1, %2, %0" : "+v"(o[i]) : "v"(x[j]), "v"(w[t]));
+                if (t >= 0 && t < KW) k3_fma2(o[i], x[j], w[t]);
             }
         }
 #pragma unroll

@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256) void k3_pair128(const P128Args A) {
 #pragma unroll
                     for (int k = 0; k < 16; k++) {
                         const int t = w - k;
-                        if (t >= 0 && t < 9) asm volatile("v_pk_fma_f32 %0, %1, %2, %0" : "+v"(o[k >> 3][k & 7]) : "v"(W[w]), "v"(tw[t]));
+                        if (t >= 0 && t < 9) k3_fma2(o[k >> 3][k & 7], W[w], tw[t]);
                     }
                 }
                 P128_T(3);
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(256) void k3_pair128(const P128Args A) {
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const int t = j - i;
-                            if (t >= 0 && t < 9) asm volatile("v_pk_fma_f32 %0, %1, %2, %0" : "+v"(o[i]) : "v"(x[j]), "v"(tw[f][t]));
+                            if (t >= 0 && t < 9) k3_fma2(o[i], x[j], tw[f][t]);
                         }
                     }
                     uint16_t *ap = &P0[s & 1][h * NCBF + f][0] + 8 * rq * CNN_BP + 2 * cpl;
