@@ -917,8 +917,9 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
 // ---- what fp16 has too few bits for, from bf16 pieces ---------------------------------------------------------------------------------------------------------------
 // One launch behind dx's and dw's, for the rows and tiles that they marked.  Ordinary gradients mark few (normal numbers, row sizes spread by a factor of e: 3 of 2000
 // tiles of 64 rows x 64 channels, next to no rows).  Bound by latency: nothing marked 3 to 5 us, 1 Mi x 256 x 256 33 us, 8192 x 4096 x 4096 47 us, both bf16.  With everything
-// marked (numbers spread evenly over 2^40) the whole gradient takes 5.3 ms and 5.5 ms instead of 0.53 and 0.66.
-// dx: a workgroup takes 64 input channels and a slice of the marks, sixteen marked rows at a time, with k8_dx_few's arithmetic.
+// marked (numbers spread evenly over 2^40) the whole gradient takes 3.3 ms and 5.5 ms instead of 0.54 and 0.66, of 100000 x 256 x 256 fp32 0.46 instead of 0.15.
+// dx: a workgroup takes 64 input channels and a slice of the marks, sixteen marked rows at a time (its wavefronts deal the output channels among themselves, or the
+// marks if there are few channels), with k8_dx_few's arithmetic.
 // dw: a workgroup takes 64 x 256 results of one run, adds up its marked tiles in steps of 64 rows, and adds that to the run's result.
 struct K8Again {
     const uint8_t *dx; int rows; int64_t units; unsigned cols, slices, dx_blocks;         // a mark of dx stands for `rows` rows
@@ -943,48 +944,62 @@ template <class T>
 __device__ __forceinline__ void k8_dx_again(const dn_i8_grad_desc &d, const K8Again &a, float (&sums)[8][4][256], int *lst, int *before) {
     const int lane = threadIdx.x & 63, wave = k8_uniform(threadIdx.x >> 6), c = lane & 15, g = lane >> 4, n = (int)d.n;
     const int64_t k0 = (int64_t)(blockIdx.x % a.cols) * 64, per = (a.units + a.slices - 1) / a.slices, u0 = (blockIdx.x / a.cols) * per, u1 = min(u0 + per, a.units);
+    // sixteen rows (a lane's is `row`) times the output channels of steps first, first + stride, ..
+    auto product = [&](int64_t row, int first, int stride, k8_f32x4 (&sum)[4]) __attribute__((always_inline)) {
+        const T *px = (const T *)d.dy + row * d.ldy;
+        const uint8_t *pm = d.mask ? d.mask + row * d.ldmask : nullptr;
+        K8Few<T> f;
+#pragma unroll
+        for (int t = 0; t < 4; t++) sum[t] = k8_f32x4{ 0, 0, 0, 0 };
+        for (int step = first; step * 64 < n; step += stride) {
+            i32x4 b[2][4];
+            unsigned codes[2][8];
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const int at = step * 64 + s * 32 + 8 * g;
+                f.bits[s] = pm ? pm[min(at, n - 1) >> 3] : 255u;
+                k8_eight_rows(d, at, k0 + 4 * c, codes[s]);
+            }
+            if (step * 64 + 64 <= n) {
+#pragma unroll
+                for (int s = 0; s < 2; s++) { f.x[s].load(px + step * 64 + s * 32 + 8 * g); f.sw[s].load(d.sw + step * 64 + s * 32 + 8 * g); }
+            } else {
+#pragma unroll
+                for (int s = 0; s < 2; s++) { const int at = step * 64 + s * 32 + 8 * g; f.x[s].load(px + at, n - at); f.sw[s].load(d.sw + at, n - at); }
+            }
+            f.pieces(true);
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                k8_columns(codes[s], b[s]);
+#pragma unroll
+                for (int t = 0; t < 4; t++) b[s][t] = k8_bf16_codes(b[s][t]);
+            }
+            f.add(b, sum);
+        }
+    };
     for (int64_t u = u0; u < u1; u += K8_MARKS) {
         const int marked = k8_marks(a.dx + u, u1 - u, lst, before);
-        for (int i0 = 0; i0 < marked; i0 += 16 / a.rows) {
-            const int m = a.rows == 16 ? (int)min(d.m - (u + lst[i0]) * 16, (int64_t)16) : min(marked - i0, 16);
-            auto place = [&](int r) { return a.rows == 16 ? (u + lst[i0]) * 16 + r : u + lst[i0 + r]; };
-            const int64_t row = place(min(c, m - 1));
-            const T *px = (const T *)d.dy + row * d.ldy;
-            const uint8_t *pm = d.mask ? d.mask + row * d.ldmask : nullptr;
-            K8Few<T> f;
-            k8_f32x4 sum[4];
+        k8_f32x4 sum[4];
+        if (a.rows == 16)                                  // few output channels: a wavefront takes a mark's rows by itself
+            for (int i = wave; i < marked; i += 8) {
+                const int64_t first = (u + k8_uniform(lst[i])) * 16;
+                product(min(first + c, d.m - 1), 0, 1, sum);
 #pragma unroll
-            for (int t = 0; t < 4; t++) sum[t] = k8_f32x4{ 0, 0, 0, 0 };
-            for (int step = wave; step * 64 < n; step += 8) {
-                i32x4 b[2][4];
-                unsigned codes[2][8];
+                for (int q = 0; q < 4; q++)                // D: column lane & 15, row 4 g + q
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    const int at = step * 64 + s * 32 + 8 * g;
-                    f.bits[s] = pm ? pm[min(at, n - 1) >> 3] : 255u;
-                    k8_eight_rows(d, at, k0 + 4 * c, codes[s]);
-                }
-                if (step * 64 + 64 <= n) {
-#pragma unroll
-                    for (int s = 0; s < 2; s++) { f.x[s].load(px + step * 64 + s * 32 + 8 * g); f.sw[s].load(d.sw + step * 64 + s * 32 + 8 * g); }
-                } else {
-#pragma unroll
-                    for (int s = 0; s < 2; s++) { const int at = step * 64 + s * 32 + 8 * g; f.x[s].load(px + at, n - at); f.sw[s].load(d.sw + at, n - at); }
-                }
-                f.pieces(true);
-#pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    k8_columns(codes[s], b[s]);
-#pragma unroll
-                    for (int t = 0; t < 4; t++) b[s][t] = k8_bf16_codes(b[s][t]);
-                }
-                f.add(b, sum);
+                    for (int t = 0; t < 4; t++)
+                        if (first + 4 * g + q < d.m && k0 + 4 * c + t < d.k) ((T *)d.dx)[(first + 4 * g + q) * d.ldx + k0 + 4 * c + t] = (T)sum[t][q];
             }
-            k8_few_join(sums, sum, m, (int)min((int64_t)64, d.k - k0), [&](int r, int kk, float v) __attribute__((always_inline)) {
-                ((T *)d.dx)[place(r) * d.ldx + k0 + kk] = (T)v;
-            });
-            __syncthreads();                               // the sums and the places are read
-        }
+        else
+            for (int i0 = 0; i0 < marked; i0 += 16) {
+                const int m = min(marked - i0, 16);
+                product(u + lst[i0 + min(c, m - 1)], wave, 8, sum);
+                k8_few_join(sums, sum, m, (int)min((int64_t)64, d.k - k0), [&](int r, int kk, float v) __attribute__((always_inline)) {
+                    ((T *)d.dx)[(u + lst[i0 + r]) * d.ldx + k0 + kk] = (T)v;
+                });
+                __syncthreads();                           // the sums are read
+            }
+        __syncthreads();                                   // the places are read
     }
 }
 template <class T>
