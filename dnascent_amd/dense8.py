@@ -100,7 +100,7 @@ def _no_gradient(**tensors):
     """the calls give tensors without a history: one that asks for a gradient would lose it without a word"""
     if torch.is_grad_enabled():
         for name, t in tensors.items():
-            if t is not None and t.requires_grad:
+            if getattr(t, "requires_grad", False):          # (what is no tensor is refused for that)
                 raise ValueError("%s requires a gradient, which this call does not pass on: use dense8.Dense, torch.no_grad() or .detach()" % name)
 
 
@@ -282,7 +282,7 @@ class Dense(torch.nn.Module):
         return new
 
     def forward(self, x, residual=None):
-        if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.weight, self.bias, residual))):
+        if not (torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (x, self.weight, self.bias, residual))):
             return _dense(self.ctx, x, self.weight, self.bias, residual, self.relu, False)[0]           # nothing to keep
         return _Layer.apply(x, self.weight, self.bias, residual, self.ctx, self.relu)
 

@@ -146,3 +146,12 @@ def test_arguments_that_require_a_gradient_are_refused():
                        ("s", lambda: dense8.restore(ctx, q, grad(s), torch.float32)), ("dy", lambda: dense8.linear_grad(ctx, grad(r), x8, sx, q, s))]:
         with pytest.raises(ValueError, match="^%s requires a gradient" % name):
             call()
+
+
+def test_arguments_that_are_no_tensors_are_type_errors():
+    ctx = SimpleNamespace(device=-1, h=None)
+    x, q, s = torch.zeros(2, 8), torch.zeros(3, 8, dtype=torch.int8), torch.zeros(3)
+    for call in (lambda: dense8.linear(ctx, x.numpy(), q, s), lambda: dense8.linear(ctx, x, q, s, bias=s.numpy()), lambda: dense8.linear(ctx, x, q, s, residual=[0.0]),
+                 lambda: dense8.linear(ctx, torch.zeros(2, 8, dtype=torch.int8), q, s, sx=s.numpy()), lambda: dense8.linear_grad(ctx, x, torch.zeros(2, 8, dtype=torch.int8), 3.0, q, s)):
+        with pytest.raises(TypeError):
+            call()
