@@ -7,7 +7,7 @@
 // That holds for values of at least 2^-14 under their power: 2^-28 of a row's largest for dx (2^-18 where k8_dx_narrow takes an upper bound for it), 2^-24 of a
 // channel's largest so far for dw.  A smaller one may be all that a result has -- the code under the large one can be zero, and half the codes behind a ReLU are --
 // so whoever meets one marks its row (k8_pieces), its sixteen rows (k8_dx_narrow) or its tile (k8_dw, which leaves it out), and k8_again makes those from bf16
-// pieces, whose exponents reach as far as fp32's: two for 16-bit results (2^-17), three for fp32 ones (2^-25), for values down to 2^-110.
+// pieces, whose exponents reach as far as fp32's: two for 16-bit results (2^-17), three for fp32 ones (2^-25), for values down to 2^-100.
 // Sums are fp32; their order depends on the sizes and on what is marked, both the same every time.
 #include "k8_dense.h"
 #include "k8_dev.h"

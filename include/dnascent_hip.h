@@ -274,7 +274,7 @@ int dn_debug_emission(dn_ctx *ctx, uint32_t n, const double *x, const double *mu
  *   its gradient:          dz = dy, zero where the forward pass's ReLU kept nothing (also where dy is NaN there); dx[m][k] = sum_n dz sw[n] w[n][k],
  *                          dw[n][k] = sum_m dz s[m] q[m][k], db[n] = sum_m dz; sums in fp32, the same bits every time.  In dx and dw the factor that carries the scale
  *                          (dz sw[n], dz s[m]) has 11 bits for 16-bit results and 22 for fp32 ones (up to 16 rows: 16 and 24, dw's 24), whatever else its row or
- *                          channel holds, for factors of at least 2^-110; rows or channels whose numbers lie more than 2^24 apart take longer
+ *                          channel holds, for factors of at least 2^-100; rows or channels whose numbers lie more than 2^24 apart take longer
  * Unlike the stages above these calls work on the CALLER's device memory (plain pointers of the context's device, rows at a pitch of ld elements),
  * are enqueued on the caller's stream (hip_stream: a hipStream_t, NULL = the default stream) and keep nothing: no allocation, no
  * synchronisation, no state in the context but the error text, so they can be captured into a graph and run on several streams at once.

@@ -922,3 +922,14 @@ def test_grad_with_channel_scales_far_apart_and_zero(ctx, m, n, k, relu, dtype):
     dead = torch.zeros_like(ws)
     dx, dw, db = ctx.i8_linear_grad(dy, q, s, wq, dead, mask=mask)
     assert not dx.any() and torch.equal(dw, got[1]) and torch.equal(db, got[2])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shift", [-75, 60])
+@pytest.mark.parametrize("m,n,k", [(300, 64, 64), (3000, 256, 256), (600, 300, 520)])
+def test_grad_of_small_terms_near_the_ends_of_the_range(ctx, m, n, k, shift, dtype):
+    """the same, with every number 2^-75 or 2^60 of what it was: factors down to 2^-100, and large ones far from fp32's end still"""
+    by_row, by_col, q, s, wq, ws, mask = _outliers(m, n, k, F32, 34, m + n)
+    for dy in (by_row, by_col):
+        dy = (dy * 2.0 ** shift).to(dtype)
+        check_grad(ctx.i8_linear_grad(dy, q, s, wq, ws, mask=mask), grad_ref(dy, q, s, wq, ws, mask), m, n, dtype, dtype)
