@@ -105,7 +105,7 @@ __device__ __forceinline__ K8Pow k8_pow(unsigned top) {
 // each row's power of two, and multiplies with the weight, whose transposed fragments lie in LDS as fp16 (256 k x N).  Nothing but dy, the mask and dx moves.
 // NP: pieces.  512 threads, so that a lane has 256 registers: enough up to N = 128, and for N = 256 all but 9 (bf16), 15 (fp16) or 58 (fp32), which go to memory; 768 threads
 // hide more but keep less (100000 x 256 x 256 with dw, bf16, us: 80 : 91; 1 Mi rows, 499 : 517).
-// 1 Mi x 256 x 256 bf16 with ReLU: 260 us; its 1.1 GB take 213 at a copy's rate, its products 104, and the vector instructions that mask, scale and convert about as long.
+// 1 Mi x 256 x 256 bf16 with ReLU: 258 us; its 1.1 GB take 213 at a copy's rate, its products 104, and the vector instructions that mask, scale and convert about as long.
 template <class T, int NS, int NP>
 __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d, uint8_t *__restrict__ again) {
     constexpr int WG = 512;
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d, uint8_t *
 // ---- dx, wide layers: the pieces of dz sw as rows of fp16, the transposed weight as rows of fp16, then k8_gemm -----------------------------------------------------
 // LPR lanes hold a row, V pieces of eight numbers each; with V = 0 they walk it twice (the second time from cache).  np: pitch in fp16, a multiple of 8; zeros behind n.
 // Two pieces: the second one's plane comes first (k8_gemm multiplies its sums with 2^-12 where the first one's begins).
-// HBM: 8192 x 4096 bf16, 22 us, 6.1 TB/s.  The weight beside it (k8_turn): 4096 x 4096, 14 us; the product: 247 us, 1.11 PFLOP/s.
+// HBM: 8192 x 4096 bf16, 23 us, 5.8 TB/s.  The weight beside it (k8_turn): 4096 x 4096, 15 us; the product: 250 us, 1.10 PFLOP/s.
 template <class T, int LPR, int V, int NP>
 __global__ __launch_bounds__(256) void k8_pieces(dn_i8_grad_desc d, _Float16 *__restrict__ out, int np, int64_t plane, float *__restrict__ down, uint8_t *__restrict__ again) {
     const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
@@ -916,7 +916,7 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
 }
 // ---- what fp16 has too few bits for, from bf16 pieces ---------------------------------------------------------------------------------------------------------------
 // One launch behind dx's and dw's, for the rows and tiles that they marked.  Ordinary gradients mark few (normal numbers, row sizes spread by a factor of e: 3 of 2000
-// tiles of 64 rows x 64 channels, next to no rows).  Bound by latency: nothing marked 3 to 5 us, 1 Mi x 256 x 256 33 us, 8192 x 4096 x 4096 47 us, both bf16.  With everything
+// tiles of 64 rows x 64 channels, next to no rows).  Bound by latency: nothing marked 2 to 5 us, 1 Mi x 256 x 256 25 us, 8192 x 4096 x 4096 43 us, both bf16.  With everything
 // marked (numbers spread evenly over 2^40) the whole gradient takes 3.3 ms and 5.5 ms instead of 0.54 and 0.66, of 100000 x 256 x 256 fp32 0.46 instead of 0.15.
 // dx: a workgroup takes 64 input channels and a slice of the marks, sixteen marked rows at a time (its wavefronts deal the output channels among themselves, or the
 // marks if there are few channels), with k8_dx_few's arithmetic.
