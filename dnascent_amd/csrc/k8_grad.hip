@@ -74,23 +74,23 @@ __device__ __forceinline__ void k8_columns(const unsigned (&d)[8], i32x4 (&out)[
             out[j][p] = __builtin_bit_cast(int, __builtin_bit_cast(k8_f16x2, t) - k8_f16x2{ (_Float16)1152.0f, (_Float16)1152.0f });
         }
 }
-// rows nn .. nn + 7 of four codes each from channel kk on, without a branch around a load: rows behind the last one repeat it (what they are multiplied with is zero),
-// four channels that end behind the matrix are read in front of its end and moved down
-__device__ __forceinline__ void k8_eight_rows(const dn_i8_grad_desc &d, int nn, int64_t kk, unsigned (&rows)[8]) {
-    if (d.k >= 4) {
-        const int64_t at = min(kk, d.k - 4);
+// rows first .. first + 7 of `n` rows, four codes each from channel kk of k on, without a branch around a load: rows behind the last one repeat it (what they are multiplied
+// with is zero), four channels that end behind the matrix are read in front of its end and moved down
+__device__ __forceinline__ void k8_eight_rows(const int8_t *__restrict__ from, int64_t ld, int64_t n, int64_t k, int64_t first, int64_t kk, unsigned (&rows)[8]) {
+    if (k >= 4) {
+        const int64_t at = min(kk, k - 4);
         const int skip = 8 * (int)min(kk - at, (int64_t)3);
 #pragma unroll
-        for (int e = 0; e < 8; e++) __builtin_memcpy(&rows[e], d.w + min((int64_t)(nn + e), d.n - 1) * d.ldw + at, 4);
+        for (int e = 0; e < 8; e++) __builtin_memcpy(&rows[e], from + min(first + e, n - 1) * ld + at, 4);
 #pragma unroll
         for (int e = 0; e < 8; e++) rows[e] >>= skip;
     } else
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const int8_t *p = d.w + min((int64_t)(nn + e), d.n - 1) * d.ldw;
+            const int8_t *p = from + min(first + e, n - 1) * ld;
             rows[e] = 0u;
 #pragma unroll
-            for (int j = 0; j < 4; j++) rows[e] |= (unsigned)(uint8_t)p[min(kk + j, d.k - 1)] << (8 * j);
+            for (int j = 0; j < 4; j++) rows[e] |= (unsigned)(uint8_t)p[min(kk + j, k - 1)] << (8 * j);
         }
 }
 // the power of two that puts `top` (bits of a magnitude, finite) into [2^14, 2^15), and its inverse; both are normal numbers
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(512) void k8_dx_narrow(dn_i8_grad_desc d, uint8_t *
     for (int f = threadIdx.x; f < blocks * NS * 64; f += WG) {
         const int fc = f & 15, fg = (f >> 4) & 3, step = (f >> 6) % NS, blk = (f >> 6) / NS, kk = blk * 64 + 4 * fc;
         unsigned rows[8];
-        k8_eight_rows(d, step * 32 + 8 * fg, k0 + kk, rows);
+        k8_eight_rows(d.w, d.ldw, d.n, d.k, step * 32 + 8 * fg, k0 + kk, rows);
         i32x4 out[4];
         k8_columns(rows, out);
 #pragma unroll
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(256) void k8_turn(dn_i8_grad_desc d, _Float16 *__re
     const int nn = (int)bn * 64 + (threadIdx.x & 7) * 8, kk = (int)bk * 128 + (threadIdx.x >> 3) * 4;
     if (nn >= np || kk >= k) return;
     unsigned rows[8];
-    k8_eight_rows(d, nn, kk, rows);
+    k8_eight_rows(d.w, d.ldw, d.n, d.k, nn, kk, rows);
     i32x4 o[4];
     k8_columns(rows, o);
 #pragma unroll
@@ -958,7 +958,7 @@ __device__ __forceinline__ void k8_dx_again(const dn_i8_grad_desc &d, const K8Ag
             for (int s = 0; s < 2; s++) {
                 const int at = step * 64 + s * 32 + 8 * g;
                 f.bits[s] = pm ? pm[min(at, n - 1) >> 3] : 255u;
-                k8_eight_rows(d, at, k0 + 4 * c, codes[s]);
+                k8_eight_rows(d.w, d.ldw, d.n, d.k, at, k0 + 4 * c, codes[s]);
             }
             if (step * 64 + 64 <= n) {
 #pragma unroll
@@ -1009,7 +1009,7 @@ __device__ __forceinline__ void k8_dw_again(const dn_i8_grad_desc &d, const K8Ag
     const int64_t t0 = z * (a.o.run / a.rt), t1 = min((z + 1) * (a.o.run / a.rt), a.o.row_tiles);
     const uint8_t *marks = a.o.again + bn * a.o.row_tiles;
     const int nt = wave >> 1, kt = (wave & 1) * 8;         // what a wavefront multiplies: 16 output channels, 128 input channels
-    const int ncols = (int)min((int64_t)64, d.n - n0), kcols = (int)min((int64_t)256, d.k - k0);
+    const int ncols = (int)min((int64_t)64, d.n - n0);
     // a channel's 64 rows: 128 bytes; its pieces of 16 bytes lie where sixteen channels' reach different banks
     auto place = [&](int channel, int piece) { return channel * 128 + ((piece ^ (channel >> 1 & 7)) << 4); };
     char *lq = lds + 3 * 8192;
@@ -1024,63 +1024,43 @@ __device__ __forceinline__ void k8_dw_again(const dn_i8_grad_desc &d, const K8Ag
             const int64_t first = (u + lst[i]) * a.rt, end = min(first + a.rt, d.m);
             for (int64_t r0 = first; r0 < end; r0 += 64) {
                 const int rows = (int)min((int64_t)64, end - r0);
-                // a thread's tasks: eight rows of four input channels, and for 128 of them of four output channels.  All of a step's numbers are asked for at once
-                const int chq = (tid & 63) * 4, rq = tid >> 6, atq = min(chq, kcols - 1), ch = (tid & 15) * 4, rg = (tid >> 4) & 7, at = min(ch, ncols - 1);
-                unsigned qs[8], bit[8];
-                K8Raw<T, 4> raw[8];
+                // a thread's tasks: eight rows of one output channel and of four input channels.  A step's numbers are asked for all at once; those behind the
+                // rows and the channels repeat the last ones and count as zeros (input channels: are not stored).  Little code: it is run by few, and fetched for each
+                const int ch = min(lane, ncols - 1);
+                T raw[8];
                 float s[8];
-                auto row = [&](int first, int e) { return r0 + min(first * 8 + e, rows - 1); };
-                if (chq + 4 <= kcols) {
+                unsigned bit[8], codes[8];
+                k8_eight_rows(d.q, d.ldq, end, d.k, r0 + wave * 8, k0 + 4 * lane, codes);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) __builtin_memcpy(&qs[e], d.q + row(rq, e) * d.ldq + k0 + chq, 4);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {          // (channels behind the last one repeat it; they are not stored)
-                        const int8_t *q = d.q + row(rq, e) * d.ldq + k0 + atq;
-                        qs[e] = 0u;
-#pragma unroll
-                        for (int j = 0; j < 4; j++) qs[e] |= (unsigned)(uint8_t)q[min(j, kcols - 1 - atq)] << (8 * j);
-                    }
+                for (int e = 0; e < 8; e++) {
+                    const int64_t r = r0 + min(wave * 8 + e, rows - 1);
+                    raw[e] = ((const T *)d.dy)[r * d.ldy + n0 + ch];
+                    s[e] = d.s[r];
+                    bit[e] = 255u;
                 }
-                if (tid < 128) {
+                if (d.mask)                                // (one branch: a load in a branch of its own is waited for there)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) { s[e] = d.s[row(rg, e)]; bit[e] = 255u; }
-                    if (d.mask)
-#pragma unroll
-                        for (int e = 0; e < 8; e++) bit[e] = d.mask[row(rg, e) * d.ldmask + ((n0 + at) >> 3)];
-                    if (ch + 4 <= ncols) {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) raw[e].load((const T *)d.dy + row(rg, e) * d.ldy + n0 + ch);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) raw[e].load((const T *)d.dy + row(rg, e) * d.ldy + n0 + at, ncols - at);
-                    }
-                }
+                    for (int e = 0; e < 8; e++) bit[e] = d.mask[(r0 + min(wave * 8 + e, rows - 1)) * d.ldmask + ((n0 + ch) >> 3)];
                 __syncthreads();                           // the last step's operands are read
-                if (tid < 128) {
+                i32x4 o[3];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {          // behind the rows and the channels: zeros
-                        bit[e] = rg * 8 + e < rows && ch < ncols ? bit[e] >> (at & 7) : 0u;
-                        if (rg * 8 + e >= rows) s[e] = 0.0f;
+                for (int p = 0; p < 4; p++) {
+                    float v[2];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int e = 2 * p + h;
+                        const bool in = wave * 8 + e < rows && lane < ncols;
+                        v[h] = (in && (bit[e] >> (ch & 7) & 1u) ? (float)raw[e] : 0.0f) * (in ? s[e] : 0.0f);
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        i32x4 o[3];
-#pragma unroll
-                        for (int p = 0; p < 4; p++) {
-                            auto value = [&](int e) { return __uint_as_float(__float_as_uint(raw[e].get(j)) & (unsigned)((int)(bit[e] << (31 - j)) >> 31)) * s[e]; };
-                            float v0 = value(2 * p), v1 = value(2 * p + 1);
-#pragma unroll
-                            for (int q = 0; q < 3; q++) o[q][p] = k8_bf16_take(v0, v1);
-                        }
-#pragma unroll
-                        for (int q = 0; q < 3; q++) *(i32x4 *)(lds + q * 8192 + place(ch + j, rg)) = o[q];
-                    }
+                    for (int i = 0; i < 3; i++) o[i][p] = k8_bf16_take(v[0], v[1]);
                 }
-                i32x4 o[4];
-                k8_columns(qs, o);
 #pragma unroll
-                for (int j = 0; j < 4; j++) *(i32x4 *)(lq + place(chq + j, rq)) = k8_bf16_codes(o[j]);
+                for (int i = 0; i < 3; i++) *(i32x4 *)(lds + i * 8192 + place(lane, wave)) = o[i];
+                i32x4 q[4];
+                k8_columns(codes, q);
+#pragma unroll
+                for (int j = 0; j < 4; j++) *(i32x4 *)(lq + place(4 * lane + j, wave)) = k8_bf16_codes(q[j]);
                 __syncthreads();
                 for (int p = a.pieces - 1; p >= 0; p--)    // the small ones first
 #pragma unroll
@@ -1101,15 +1081,17 @@ __device__ __forceinline__ void k8_dw_again(const dn_i8_grad_desc &d, const K8Ag
     for (int t = 0; t < 8; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) run[t][i] = part[min((int64_t)i, d.n - 1 - nn) * d.k + min((int64_t)t * 16, d.k - 1 - kk)];
+    auto put = [&](auto *to, int64_t pitch) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < 8; t++)
+        for (int t = 0; t < 8; t++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (nn + i >= d.n || kk + t * 16 >= d.k) continue;
-            const float v = run[t][i] + acc[t][i];
-            if (a.o.splits > 1) part[i * d.k + t * 16] = v;
-            else k8_put1(d.dw, d.dw_type, (nn + i) * d.lddw + kk + t * 16, v);
-        }
+            for (int i = 0; i < 4; i++)
+                if (nn + i < d.n && kk + t * 16 < d.k) to[(nn + i) * pitch + kk + t * 16] = (std::remove_pointer_t<decltype(to)>)(run[t][i] + acc[t][i]);
+    };
+    if (a.o.splits > 1) put(a.o.part + z * d.n * d.k, d.k);
+    else if (d.dw_type == DN_T_F32) put((float *)d.dw, d.lddw);
+    else if (d.dw_type == DN_T_F16) put((_Float16 *)d.dw, d.lddw);
+    else put((k8_bf16 *)d.dw, d.lddw);
 }
 template <class T>
 __global__ __launch_bounds__(512) void k8_again(dn_i8_grad_desc d, K8Again a) {
