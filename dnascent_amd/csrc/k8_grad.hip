@@ -916,7 +916,7 @@ __global__ __launch_bounds__(512) void k8_dw(dn_i8_grad_desc d, DwOut o) {
 }
 // ---- what fp16 has too few bits for, from bf16 pieces ---------------------------------------------------------------------------------------------------------------
 // One launch behind dx's and dw's, for the rows and tiles that they marked.  Ordinary gradients mark few (normal numbers, row sizes spread by a factor of e: 3 of 2000
-// tiles of 64 rows x 64 channels, next to no rows).  Bound by latency: nothing marked 2 to 5 us, 1 Mi x 256 x 256 25 us, 8192 x 4096 x 4096 43 us, both bf16.  With everything
+// tiles of 64 rows x 64 channels, next to no rows).  Bound by latency: nothing marked 2 to 5 us, 1 Mi x 256 x 256 24 us, 8192 x 4096 x 4096 35 us, both bf16.  With everything
 // marked (numbers spread evenly over 2^40) the whole gradient takes 3.3 ms and 5.5 ms instead of 0.54 and 0.66, of 100000 x 256 x 256 fp32 0.46 instead of 0.15.
 // dx: a workgroup takes 64 input channels and a slice of the marks, sixteen marked rows at a time (its wavefronts deal the output channels among themselves, or the
 // marks if there are few channels), with k8_dx_few's arithmetic.
